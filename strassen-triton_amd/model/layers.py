@@ -138,9 +138,12 @@ def replace_linear_with_strassen(module: nn.Module, min_size: int = 128, depth: 
     square_only=False every layer whose smaller side is at least min_size becomes a
     LinearStrassenRect instead (any shape, any number of input rows -- the reference's layer
     refuses more than D rows); below min_size a layer stays an nn.Linear, i.e. a classical GEMM.
+    A LinearAct stays too: no Strassen layer has its activation, nor takes a residual.
     cache_weight_sums and cutoff are handed to the new layers (cutoff: see LinearStrassenRect)."""
     for name, child in module.named_children():
-        if isinstance(child, nn.Linear) and not isinstance(child, (_LinearStrassen, LinearStrassenRect)):
+        if isinstance(child, LinearAct):
+            print(f"Skipping '{name}': a product with an epilogue.")
+        elif isinstance(child, nn.Linear) and not isinstance(child, (_LinearStrassen, LinearStrassenRect)):
             if not square_only and min(child.in_features, child.out_features) >= min_size:
                 print(f"Replacing '{name}' with LinearStrassenRect.")
                 new_layer = LinearStrassenRect(child.in_features, child.out_features,
