@@ -285,25 +285,59 @@ struct Rotary : torch::autograd::Function<Rotary> {
     }
 };
 
-// Whether two elements may share memory: sorted by stride, each dimension has to step over all smaller ones.
+// Whether integers within their bounds give sum(step * number) = target.  Terms in descending order of their steps (all positive): of
+// each only those numbers are tried whose rest the terms behind it can reach, one or two where strides nest.  Yes where `tries` run out.
+struct Term { int64_t step, lo, hi; };
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+bool reaches(const Term* t, const Term* end, int64_t target, int& tries) {
+    if (t == end) return target == 0;
+    if (--tries < 0) return true;
+    int64_t lo = 0, hi = 0;   // of the terms behind
+    for (const Term* r = t + 1; r != end; ++r) lo += r->step * r->lo, hi += r->step * r->hi;
+    const int64_t last = std::min(t->hi, floor_div(target - lo, t->step));
+    for (int64_t n = std::max(t->lo, -floor_div(hi - target, t->step)); n <= last; ++n)
+        if (reaches(t + 1, end, target - n * t->step, tries)) return true;
+    return false;
+}
+constexpr int kTries = 100000;   // a millisecond
+bool descending(const Term& a, const Term& b) { return a.step > b.step; }
+
+// Whether two elements share memory: their indices differ, first in some dimension and there by a positive number.
 bool overlaps_itself(const Tensor& t) {
-    std::vector<std::pair<int64_t, int64_t>> d;
-    for (int64_t i = 0; i < t.dim(); ++i) if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
-    std::sort(d.begin(), d.end());
-    int64_t reach = 0;
-    for (auto& [stride, size] : d) {
-        if (stride <= reach) return true;
-        reach += stride * (size - 1);
+    std::vector<Term> d;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) == 0) return false;
+        if (t.size(i) > 1) d.push_back({t.stride(i), 1 - t.size(i), t.size(i) - 1});
+    }
+    std::sort(d.begin(), d.end(), descending);
+    if (!d.empty() && d.back().step == 0) return true;
+    int tries = kTries;
+    for (size_t i = 0; i < d.size(); ++i) {
+        const int64_t lo = std::exchange(d[i].lo, 1);
+        if (reaches(d.data() + i, d.data() + d.size(), 0, tries)) return true;
+        d[i].lo = lo;
     }
     return false;
 }
 
-// Whether q and k of one packed tensor (the same strides) have a head in common; of others, whether they start at one place.
+// Whether an element of q and one of k share memory: byte q + sum(index * stride) + byte of the element = the same of k.
 bool share(const Tensor& q, const Tensor& k) {
     if (!q.numel() || !k.numel()) return false;
-    if (q.data_ptr() == k.data_ptr()) return true;
-    const int64_t apart = ((const char*)k.data_ptr() - (const char*)q.data_ptr()) / (int64_t)q.element_size();
-    return q.strides() == k.strides() && apart < (q.size(2) - 1) * q.stride(2) + q.size(3) && -apart < (k.size(2) - 1) * k.stride(2) + k.size(3);
+    const int64_t es = q.element_size();
+    std::vector<Term> d = {{1, 1 - es, es - 1}};
+    auto add = [&](const Tensor& t, int sign) {
+        for (int64_t i = 0; i < t.dim(); ++i) {
+            const int64_t step = t.stride(i) * es, most = sign * (t.size(i) - 1);
+            if (most == 0 || step == 0) continue;
+            auto same = std::find_if(d.begin(), d.end(), [&](const Term& u) { return u.step == step; });
+            if (same == d.end()) same = d.insert(d.end(), {step, 0, 0});
+            (most < 0 ? same->lo : same->hi) += most;
+        }
+    };
+    add(q, 1), add(k, -1);
+    std::sort(d.begin(), d.end(), descending);
+    int tries = kTries;
+    return reaches(d.data(), d.data() + d.size(), (const char*)k.data_ptr() - (const char*)q.data_ptr(), tries);
 }
 
 std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& freq, const Maybe& pos, bool interleaved, double gain, int64_t first, bool inplace) {
@@ -376,4 +410,5 @@ PYBIND11_MODULE(_sthip_torch, m) {
     m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
     m.def("rotary", &rotary, py::arg("q"), py::arg("k"), py::arg("frequencies"), py::arg("positions"), py::arg("interleaved"), py::arg("gain"), py::arg("first"), py::arg("inplace"));
     m.def("overlaps_itself", &overlaps_itself);
+    m.def("share", &share);
 }

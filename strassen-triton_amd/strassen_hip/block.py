@@ -98,8 +98,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, frequencies: torch.Tensor, p
     head turn, the others are copied; layout "half" pairs i with i + len(frequencies), "interleaved" 2 i with 2 i + 1.
     frequencies, gain: rotary_frequencies.  positions: int32 or int64, (tokens,) or (batch, tokens); None counts from
     first_position.  Angles are formed in 64 bits: below 2^29 radians they keep
-    fp32's accuracy, beyond they are off by their size times 2^-53.  inplace=True turns q and k where they lie (any
-    strides; no gradient).  Returns (q, k), or q alone where k is None."""
+    fp32's accuracy, beyond they are off by their size times 2^-53.  inplace=True turns q and k where they lie, without a
+    gradient: unit stride within a head, any other strides, and no element twice, neither within a tensor nor in both
+    (ValueError).  Returns (q, k), or q alone where k is None."""
     try:
         interleaved = _LAYOUTS[layout]
     except KeyError:

@@ -43,3 +43,104 @@ def test_fused_block_after_the_swap():
             before = block(x)
             replace_linear_with_strassen(block, square_only=square_only)
             assert torch.equal(block(x), before)
+
+
+# ------------------------------------------------------------------------------------- rotary on memory that is shared
+def _packed(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def _pairs():
+    """(q, k, whether they have an element in common)"""
+    t, h, p, a = _packed(2, 9, 8, 16), _packed(2, 9, 4, 3, 16), _packed(2, 9, 8, 16), _packed(3, 10, 6, 16)
+    return [
+        (t[:, :, :4], t[:, :, 4:6], False), (t[:, :, :4], t[:, :, 3:6], True), (t[:, :, ::2], t[:, :, 1::2], False), (t[:, :, ::2], t[:, :, 2::4], True),
+        (t[:, :-1], t[:, 1:], True), (t[:, :4], t[:, 4:], False), (t[:, :5], t[:, 4:], True), (t[:1], t[1:], False), (t, t, True),
+        (h[:, :, :, 0], h[:, :, :, 1], False), (h[:, :, :, 1], h[:, :, :, 0], False), (h[:, :, :, 0], h[:, :, 2:, 0], True), (h[:, :, :2, 2], h[:, :, 1:, 2], True),
+        (p[:, :, :4], p[:, :, 3:8:2], True), (p[:, :, :4], p[:, :, 4:8:2], False), (p[:, :, 1:8:2], p[:, :, ::4], False), (p[:, ::2], p[:, 1::2][:, :, ::2], False),
+        (p[..., :8], p[..., 8:], False), (p[..., :9], p[..., 8:], True), (t, p, False), (a.transpose(1, 2)[:, :2], a.transpose(1, 2)[:, 2:], False),
+        (a[:, ::3], a[:, 1::3], False), (a[:, ::3], a[:, ::2], True), (a[:, 1::4], a[:, ::2], False), (a[:, :0], a, False),
+        (t[:, :1].expand(2, 9, 8, 16), t[:, 1:], False), (t[:, :1].expand(2, 9, 8, 16), t[:, :2], True),
+    ]
+
+
+def _bytes(t):
+    """Every byte of a tensor's elements."""
+    at = torch.zeros((), dtype=torch.int64)
+    for n, s in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    es = t.element_size()
+    return set((t.data_ptr() + es * at.flatten()[:, None] + torch.arange(es)).flatten().tolist())
+
+
+def test_memory_in_common():
+    from strassen_hip.block import _ext
+    share = _ext().share
+    for i, (q, k, want) in enumerate(_pairs()):
+        assert bool(_bytes(q) & _bytes(k)) == want, i   # the table itself
+        assert share(q, k) == want and share(k, q) == want, i
+
+
+def test_memory_in_common_of_any_strides():
+    """Small random strides and places, elements of two and four bytes that may begin inside one another."""
+    import random
+    from strassen_hip.block import _ext
+    share, overlaps_itself = _ext().share, _ext().overlaps_itself
+    rng, seen = random.Random(5), [0, 0, 0, 0]
+    raw = bytearray(4096)
+    for _ in range(3000):
+        dtype = rng.choice((torch.bfloat16, torch.float32))
+        views = []
+        for _ in range(2):
+            base = torch.frombuffer(raw, dtype=dtype, count=1024 - 2, offset=rng.choice((0, 0, 0, 1, 2)))
+            views.append(torch.as_strided(base, [rng.randint(1, 4) for _ in range(4)], [rng.choice((1, 2, 3, 5, 8, 12, 31, 60)) for _ in range(4)], rng.randint(0, 300)))
+        q, k = views
+        want = bool(_bytes(q) & _bytes(k))
+        assert share(q, k) == want, (q.shape, q.stride(), k.shape, k.stride())
+        itself = len(_bytes(q)) < q.numel() * q.element_size()
+        assert overlaps_itself(q) == itself, (q.shape, q.stride())
+        seen[want] += 1
+        seen[2 + itself] += 1
+    assert min(seen) > 200
+
+
+def test_memory_in_common_of_long_tensors_is_quick():
+    """Strides that do not nest in one another: an answer after a bounded number of steps, yes where they run out."""
+    import time
+    from strassen_hip.block import _ext
+    t = torch.zeros(8, 4096, 6, 16, dtype=torch.bfloat16)
+    start = time.perf_counter()
+    assert not _ext().share(t[:, :, :4], t[:, :, 4:]) and not _ext().share(t[:, ::2], t[:, 1::2])
+    assert _ext().share(t[:, ::5], t[:, 4095 // 3::7])
+    odd = torch.zeros(1 << 22, dtype=torch.bfloat16)
+    _ext().share(torch.as_strided(odd, (97, 101, 103), (9973, 9967, 7)), torch.as_strided(odd, (89, 83, 79), (9949, 9941, 11), 3))
+    assert time.perf_counter() - start < 1.0
+
+
+@pytest.mark.gpu
+def test_rotary_in_place_on_views():
+    """What has no element in common turns in place, whatever its strides; the rest is refused and left as it was."""
+    import strassen_hip as hip
+    f, _ = hip.rotary_frequencies(8)
+    for i, (q, k, common) in enumerate(_pairs()):
+        if q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+            continue
+        size = lambda t: 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+        low = min(q.data_ptr(), k.data_ptr())
+        whole = (max(q.data_ptr() + 2 * size(q), k.data_ptr() + 2 * size(k)) - low) // 2
+        if whole > 1 << 20:   # two tensors
+            continue
+        buf = _randn((whole,), torch.bfloat16, i).cuda()
+        gq, gk = (torch.as_strided(buf, t.shape, t.stride(), (t.data_ptr() - low) // 2) for t in (q, k))
+        before, (wq, wk) = buf.clone(), hip.rotary(gq, gk, f)
+        if common or 0 in gq.stride():
+            with pytest.raises(ValueError, match="share memory"):
+                hip.rotary(gq, gk, f, inplace=True)
+            assert torch.equal(buf, before)
+            continue
+        hip.rotary(gq, gk, f, inplace=True)
+        assert torch.equal(gq, wq) and torch.equal(gk, wk), i
+        rest = torch.ones_like(buf, dtype=torch.bool)
+        for t in (q, k):
+            torch.as_strided(rest, t.shape, t.stride(), (t.data_ptr() - low) // 2).fill_(False)
+        assert torch.equal(buf[rest], before[rest]), i
