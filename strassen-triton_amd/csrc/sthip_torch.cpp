@@ -69,6 +69,13 @@ Tensor with_last(const Tensor& y, const Tensor& x, int64_t cols) {
     return y.view(s);
 }
 
+// What a node saved, as the backward pass finds it: a hook on saved tensors may give back other strides, or another tensor.
+Tensor restored(const Tensor& t, const char* what, at::IntArrayRef sizes, at::ScalarType type, const Tensor& grad) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == grad.device(), "the saved ", what, " came back as ", t.toString(), " of ",
+                t.sizes(), " on ", t.device(), ", expected ", type, " of ", sizes, " on ", grad.device());
+    return t;
+}
+
 // What a backward pass returns, where it was asked for a graph of itself: tensors that refuse to be differentiated again.
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -111,13 +118,13 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         Tensor y = linear_forward(x, w, b, r, act, keep ? &pre : nullptr);
         ctx->save_for_backward({x, w, pre});
         ctx->saved_data["act"] = act;
+        ctx->saved_data["in"] = x.size(1);
         ctx->saved_data["given"] = (int64_t)((b ? 1 : 0) | (r ? 2 : 0));
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &pre = saved[2];
-        const int64_t act = ctx->saved_data["act"].toInt(), rows = x.size(0), in = x.size(1), out = w.size(0);
+        const int64_t act = ctx->saved_data["act"].toInt(), rows = grads[0].size(0), in = ctx->saved_data["in"].toInt(), out = grads[0].size(1);
         // needs_input_grad counts the tensors that were given
         const int64_t given = ctx->saved_data["given"].toInt();
         const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
@@ -125,9 +132,12 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         Tensor dx, dw, db;
         if (nx || nw || nb) {
             const at::NoGradGuard no_grad;
-            const On on(x);
+            const On on(grads[0]);
+            const auto type = grads[0].scalar_type();
+            const Tensor x = rows_of(restored(saved[0], "input", {rows, in}, type, grads[0])), w = rows_of(restored(saved[1], "weight", {out, in}, type, grads[0]));
+            const Tensor pre = act ? restored(saved[2], "pre-activation", {rows, out}, type, grads[0]).contiguous() : Tensor();
             const Tensor dy = rows_of(grads[0]);
-            const int dt = dtype_code(x.scalar_type());
+            const int dt = dtype_code(type);
             if (nx) dx = at::empty({rows, in}, x.options());
             if (nw) dw = at::empty({out, in}, x.options());
             if (nb) db = at::empty({out}, x.options());
@@ -188,16 +198,18 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
         const auto params = (at::ScalarType)ctx->saved_data["params"].toInt();
+        const int64_t rows = grads[0].size(0), cols = grads[0].size(1);
         const int64_t given = ctx->saved_data["given"].toInt();
         const bool nx = ctx->needs_input_grad(0), nw = (given & 1) && ctx->needs_input_grad(1);
         const bool nb = (given & 2) && ctx->needs_input_grad(given & 1 ? 2 : 1);
-        const int64_t rows = x.size(0), cols = x.size(1);
         Tensor dx, dw, db;
         {
             const at::NoGradGuard no_grad;
-            const On on(x);
+            const On on(grads[0]);
+            const Tensor x = rows_of(restored(saved[0], "input", {rows, cols}, grads[0].scalar_type(), grads[0]));
+            const Tensor w = given & 1 ? restored(saved[1], "weight", {cols}, params, grads[0]).contiguous() : Tensor();
+            const Tensor stats = restored(saved[2], "statistics", {2, rows}, at::kFloat, grads[0]).contiguous();
             const Tensor dy = rows_of(grads[0]);
             if (nx) dx = at::empty({rows, cols}, x.options());
             if (nw) dw = at::empty({cols}, x.options().dtype(params));
@@ -238,14 +250,16 @@ Tensor layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
 }
 
 // ---------------------------------------------------------------------------------------------------- rotary
-struct RotaryHow { int64_t pos_batch, pos_token, first; double gain; int64_t interleaved; };
+struct RotaryHow { int64_t first; double gain; int64_t interleaved; };
 
+// pos: (tokens,) or (batch, tokens), or not given.
 void rotary_into(const Tensor& q, const Tensor& k, const Tensor& qo, const Tensor& ko, const Tensor& freq, const Maybe& pos, const RotaryHow& h, int inverse) {
     const On on(q);
-    const bool two = k.defined();
+    const bool two = k.defined(), given = pos && pos->defined();
+    const int64_t pos_batch = given && pos->dim() == 2 ? pos->stride(0) : 0, pos_token = given ? pos->stride(-1) : 0;
     check(sthip_rotary(q.data_ptr(), ptr(k), qo.data_ptr(), ptr(ko), q.size(0), q.size(1), q.size(2), two ? k.size(2) : 0, q.size(3), 2 * freq.size(0),
                        q.strides().data(), two ? k.strides().data() : nullptr, qo.strides().data(), two ? ko.strides().data() : nullptr,
-                       freq.data_ptr<double>(), ptr(pos), pos && pos->defined() ? (int)pos->element_size() * 8 : 0, h.pos_batch, h.pos_token, h.first,
+                       freq.data_ptr<double>(), ptr(pos), given ? (int)pos->element_size() * 8 : 0, pos_batch, pos_token, h.first,
                        h.gain, (int)h.interleaved, inverse, dtype_code(q.scalar_type()), on.stream));
 }
 Tensor unit_heads(const Tensor& t) { return !t.defined() || t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
@@ -257,7 +271,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
         Tensor qo = like(q), ko = like(kt);
         rotary_into(q, kt, qo, ko, freq, pos, h, 0);
         ctx->save_for_backward({freq, pos ? *pos : Tensor()});
-        ctx->saved_data["how"] = std::vector<int64_t>{h.pos_batch, h.pos_token, h.first, h.interleaved};
+        ctx->saved_data["how"] = std::vector<int64_t>{h.first, h.interleaved, freq.size(0), pos ? (int64_t)pos->scalar_type() : -1, pos ? pos->dim() : 0};
         ctx->saved_data["gain"] = h.gain;
         ctx->set_materialize_grads(false);
         if (k) return {qo, ko};
@@ -266,7 +280,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
         const auto v = ctx->saved_data["how"].toIntVector();
-        const RotaryHow h = {v[0], v[1], v[2], ctx->saved_data["gain"].toDouble(), v[3]};
+        const RotaryHow h = {v[0], ctx->saved_data["gain"].toDouble(), v[1]};
         variable_list out(5), in, turned;
         int at[2], n = 0;
         {
@@ -277,7 +291,10 @@ struct Rotary : torch::autograd::Function<Rotary> {
                 const c10::DeviceGuard guard(in[0].device());
                 for (auto& t : in) turned.push_back(like(t));
                 in.resize(2), turned.resize(2);
-                rotary_into(in[0], in[1], turned[0], turned[1], saved[0], saved[1].defined() ? Maybe(saved[1]) : Maybe(), h, 1);
+                const Tensor freq = restored(saved[0], "frequencies", {v[2]}, at::kDouble, in[0]).contiguous();
+                Maybe pos;
+                if (v[4]) pos = restored(saved[1], "positions", in[0].sizes().slice(2 - v[4], v[4]), (at::ScalarType)v[3], in[0]);
+                rotary_into(in[0], in[1], turned[0], turned[1], freq, pos, h, 1);
             }
         }
         for (int i = 0; i < n; ++i) out[at[i]] = turned[i];
@@ -353,14 +370,11 @@ std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& 
     const bool flat = d == 3;
     Tensor q4 = flat ? q.unsqueeze(0) : q, k4 = !k ? Tensor() : flat ? k->unsqueeze(0) : *k;
     const int64_t batch = q4.size(0), tokens = q4.size(1);
-    RotaryHow h = {0, 0, first, gain, interleaved};
+    const RotaryHow h = {first, gain, interleaved};
     if (pos) {
         TORCH_CHECK_TYPE(pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong, "positions must be int32 or int64, got ", pos->scalar_type());
-        if (pos->dim() == 1 && pos->size(0) == tokens) h.pos_token = pos->stride(0);
-        else {
-            TORCH_CHECK_VALUE(!flat && pos->dim() == 2 && pos->size(0) == batch && pos->size(1) == tokens, "positions have shape ", pos->sizes(), ", expected [", tokens, "] or [", batch, ", ", tokens, "]");
-            h.pos_batch = pos->stride(0), h.pos_token = pos->stride(1);
-        }
+        TORCH_CHECK_VALUE((pos->dim() == 1 && pos->size(0) == tokens) || (!flat && pos->dim() == 2 && pos->size(0) == batch && pos->size(1) == tokens),
+                          "positions have shape ", pos->sizes(), ", expected [", tokens, "] or [", batch, ", ", tokens, "]");
     }
     TORCH_CHECK(!freq.requires_grad(), "rotary has no gradient for its frequencies");
     const Tensor f = freq.contiguous();

@@ -144,3 +144,64 @@ def test_rotary_in_place_on_views():
         for t in (q, k):
             torch.as_strided(rest, t.shape, t.stride(), (t.data_ptr() - low) // 2).fill_(False)
         assert torch.equal(buf[rest], before[rest]), i
+
+
+# -------------------------------------------------------------------------------------------------- hooks of autograd
+def _operators(hip, seed=1):
+    """name: (call, leaves): each operator on operands that are views with strides of their own."""
+    wide = lambda shape, pad, s: _randn((*shape[:-1], shape[-1] + pad), torch.float32, seed + s).cuda()[..., :shape[-1]].detach().requires_grad_()
+    f, _ = hip.rotary_frequencies(8)
+    x, w, b, r, n = wide((5, 24), 3, 1), wide((40, 24), 5, 2), wide((40,), 0, 3), wide((5, 40), 4, 4), wide((24,), 0, 5)
+    q, k = wide((2, 7, 3, 16), 2, 6), wide((2, 7, 1, 16), 4, 7)
+    pos = torch.randint(0, 1000, (2, 70), generator=torch.Generator().manual_seed(seed)).cuda()[:, 3:66:9]   # (2, 7), strides 70 and 9
+    return {"linear_act": (lambda: hip.linear_act(x, w, b, activation="gelu", residual=r), [x, w, b, r]), "layer_norm": (lambda: hip.layer_norm(x, n, n), [x, n]),
+            "rotary": (lambda: torch.cat(hip.rotary(q, k, f, pos), 2), [q, k])}
+
+
+def _turned(t):
+    """The same values, the first dimension's elements side by side."""
+    return t.transpose(0, -1).contiguous().transpose(0, -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["linear_act", "layer_norm", "rotary"])
+def test_saved_tensors_come_back_otherwise(name):
+    """Hooks on saved tensors: to host memory and back, in another order, by checkpoints that compute them again.  What does not come back is said."""
+    import strassen_hip as hip
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+    call, leaves = _operators(hip)[name]
+    y = call()
+    dy = _randn(tuple(y.shape), torch.float32, 9).cuda()
+    want = torch.autograd.grad(y, leaves, dy)
+    keep = lambda t: t
+    for hooks in (save_on_cpu(), saved_tensors_hooks(keep, _turned), saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda())):
+        with hooks:
+            y = call()
+        for got, ref_ in zip(torch.autograd.grad(y, leaves, dy), want):
+            assert torch.equal(got, ref_)
+    for got, ref_ in zip(torch.autograd.grad(checkpoint(lambda _: call(), leaves[0], use_reentrant=False), leaves, dy), want):
+        assert torch.equal(got, ref_)
+    for spoil in (lambda t: t.cpu(), lambda t: t[..., :1] if t.shape[-1] > 1 else t, lambda t: t.float() if t.dtype == torch.float64 else t.double()):
+        with saved_tensors_hooks(keep, spoil):
+            y = call()
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["linear_act", "layer_norm", "rotary"])
+def test_gradients_in_another_order(name):
+    """A hook on the result gives its gradient other strides, or one value for all of it."""
+    import strassen_hip as hip
+    call, leaves = _operators(hip)[name]
+    y = call()
+    dy = _randn(tuple(y.shape), torch.float32, 9).cuda()
+    want = torch.autograd.grad(y, leaves, dy)
+    y = call()
+    y.register_hook(_turned)
+    for got, ref_ in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(got, ref_)
+    one = torch.full((), 0.5).cuda()
+    for got, ref_ in zip(torch.autograd.grad(call(), leaves, one.expand(y.shape)), torch.autograd.grad(call(), leaves, one.expand(y.shape).contiguous())):
+        assert torch.equal(got, ref_)
