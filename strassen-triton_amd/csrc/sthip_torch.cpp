@@ -5,7 +5,10 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
@@ -38,6 +41,19 @@ int dtype_code(at::ScalarType t) {
 }
 void require_gpu(const Tensor& t) {
     TORCH_CHECK(t.is_cuda(), "strassen_hip runs on MI355X tensors only (got a tensor on ", t.device(), "); there is no CPU implementation in this library");
+}
+// What torch would follow through its own operations and cannot follow into these: a tangent (forward-mode derivative), a transform's
+// wrapped tensor, a program that is being recorded.  All three would get a result as if it were a constant.
+template <class Tensors> void refuse_transforms(const Tensors& tensors) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !(c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)), "the operators of strassen_hip cannot be traced");
+    const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Maybe& t : tensors) {
+        if (!t || !t->defined()) continue;
+        TORCH_CHECK(!t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched})),
+                    "the operators of strassen_hip have no torch.func transforms");
+        TORCH_CHECK(!tangents || !t->_fw_grad(0).defined(), "the operators of strassen_hip have no forward-mode derivatives");
+    }
 }
 void same_device(const Tensor& first, const Maybe& t) {
     if (t) TORCH_CHECK(t->device() == first.device(), "tensors on different devices: ", first.device(), " and ", t->device());
@@ -123,6 +139,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_transforms(grads);
         const variable_list saved = ctx->get_saved_variables();
         const int64_t act = ctx->saved_data["act"].toInt(), rows = grads[0].size(0), in = ctx->saved_data["in"].toInt(), out = grads[0].size(1);
         // needs_input_grad counts the tensors that were given
@@ -151,6 +168,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 };
 
 Tensor linear_act(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act) {
+    refuse_transforms(std::initializer_list<Maybe>{x, w, b, r});
     require_gpu(x);
     same_device(x, w), same_device(x, b), same_device(x, r);
     TORCH_CHECK_VALUE(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1), "shape mismatch: ", x.sizes(), " @ ", w.sizes(), "^T");
@@ -197,6 +215,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_transforms(grads);
         const variable_list saved = ctx->get_saved_variables();
         const auto params = (at::ScalarType)ctx->saved_data["params"].toInt();
         const int64_t rows = grads[0].size(0), cols = grads[0].size(1);
@@ -225,6 +244,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
+    refuse_transforms(std::initializer_list<Maybe>{x, w, b});
     require_gpu(x);
     same_device(x, w), same_device(x, b);
     TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm needs at least one dimension");
@@ -278,6 +298,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
         return {qo};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_transforms(grads);
         const variable_list saved = ctx->get_saved_variables();
         const auto v = ctx->saved_data["how"].toIntVector();
         const RotaryHow h = {v[0], ctx->saved_data["gain"].toDouble(), v[1]};
@@ -358,6 +379,7 @@ bool share(const Tensor& q, const Tensor& k) {
 }
 
 std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& freq, const Maybe& pos, bool interleaved, double gain, int64_t first, bool inplace) {
+    refuse_transforms(std::initializer_list<Maybe>{q, k, freq, pos});
     require_gpu(q);
     same_device(q, k), same_device(q, freq), same_device(q, pos);
     const int64_t d = q.dim();

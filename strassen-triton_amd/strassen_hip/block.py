@@ -5,8 +5,9 @@ gradients.  The reference leaves them to torch (model/model.py:4-32, model/layer
 Argument checks, memory and the autograd nodes are in csrc/sthip_torch.cpp (module _sthip_torch).  As in ops.py torch supplies
 device memory, streams and the autograd graph only, and there is no CPU path.  Calls run on the current stream of their
 tensors' device; workspaces come from torch's allocator at every call, so captured graphs share none.  Wrong arguments raise
-ValueError or TypeError, a failing C-ABI call SthipError; gradients cannot be differentiated again.  Under capture, a leaf
-that a living eager graph on the default stream uses is refused (RuntimeError): torch's engine would end the process over it.
+ValueError or TypeError, a failing C-ABI call SthipError; gradients cannot be differentiated again.  Forward-mode derivatives,
+torch.func transforms and traces are refused (RuntimeError): the operators would count as constants in them.  Under capture, a
+leaf that a living eager graph on the default stream uses is refused (RuntimeError): torch's engine would end the process over it.
 """
 from __future__ import annotations
 

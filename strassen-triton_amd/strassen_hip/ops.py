@@ -156,7 +156,9 @@ class StrassenMatmul(torch.autograd.Function):
 
 
 def matmul(A: torch.Tensor, B: torch.Tensor, algo="strassen", levels: int = 1, schedule: str = "auto") -> torch.Tensor:
-    """Differentiable A @ B."""
+    """Differentiable A @ B.  Forward-mode derivatives and traces, which would take the product for a constant, are refused."""
+    if torch.jit.is_tracing() or any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in (A, B)):
+        raise RuntimeError("the products of strassen_hip have no forward-mode derivatives and cannot be traced")
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad):
         return StrassenMatmul.apply(A, B, algo, levels, schedule)
     return gemm(A, B, algo=algo, levels=levels, schedule=schedule)

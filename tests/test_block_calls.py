@@ -205,3 +205,58 @@ def test_gradients_in_another_order(name):
     one = torch.full((), 0.5).cuda()
     for got, ref_ in zip(torch.autograd.grad(call(), leaves, one.expand(y.shape)), torch.autograd.grad(call(), leaves, one.expand(y.shape).contiguous())):
         assert torch.equal(got, ref_)
+
+
+# ------------------------------------------------------------------------------- forward mode, transforms, recorded programs
+def _entries(hip, device):
+    """Each entry point as a function of one tensor (4, 8)."""
+    w, f = torch.ones(8, 8, device=device), torch.ones(2, dtype=torch.float64, device=device)
+    return [lambda x: hip.linear_act(x, w), lambda x: hip.linear_act(w, x), lambda x: hip.linear_act(w, w, x[0]), lambda x: hip.linear_act(w[:4], w, residual=x),
+            lambda x: hip.layer_norm(x), lambda x: hip.layer_norm(w, x[0]), lambda x: hip.layer_norm(w, None, x[0]),
+            lambda x: hip.rotary(x.view(1, 2, 2, 8), None, f), lambda x: hip.rotary(w.view(1, 2, 4, 8), x.view(1, 2, 2, 8), f)[1], lambda x: hip.matmul(x, w), lambda x: hip.matmul(w[:, :4], x)]
+
+
+@pytest.mark.parametrize("i", range(11))
+def test_forward_mode_and_traces_are_refused(i):
+    """Refused before anything else is looked at: no GPU is needed to see it."""
+    import strassen_hip as hip
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    entry = _entries(hip, "cpu")[i]
+    x = _randn((4, 8), torch.float32, 1)
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no forward-mode"):
+            entry(dual)
+        if i < 9:   # as in torch's own operations, there is no tangent where they are switched off
+            with torch.inference_mode(), pytest.raises(RuntimeError, match="no CPU implementation"):
+                entry(dual)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(entry, (x,), check_trace=False)
+    if i < 9:
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(entry)(x)
+        with pytest.raises(RuntimeError, match="no torch.func|no forward-mode"):
+            torch.func.jvp(entry, (x,), (x,))
+        with pytest.raises(RuntimeError, match="no torch.func"):
+            torch.func.vmap(lambda u: entry(u))(x[None])
+        with pytest.raises(RuntimeError, match="no torch.func"):
+            torch.func.grad(lambda u: entry(u).sum())(x)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        entry(x)
+
+
+@pytest.mark.gpu
+def test_forward_mode_over_gradients_is_refused():
+    import strassen_hip as hip
+    import torch.autograd.forward_ad as forward_ad
+    for name, (call, leaves) in _operators(hip).items():
+        y = call()
+        dy = torch.ones_like(y)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode"):
+            torch.autograd.grad(y, leaves, forward_ad.make_dual(dy, dy))
+    for entry in _entries(hip, "cuda"):
+        x = _randn((4, 8), torch.float32, 1).cuda()
+        with forward_ad.dual_level():   # a level without a tangent changes nothing
+            got = entry(x)
+        assert torch.equal(got, entry(x))
