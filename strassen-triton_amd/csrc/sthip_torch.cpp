@@ -11,6 +11,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <unordered_set>
 
 #include "../../include/strassen_hip.h"
 
@@ -101,16 +102,27 @@ variable_list once(variable_list grads) {
     return (*node)(std::move(fake));
 }
 
-// A leaf that a living eager graph uses keeps its accumulation on that graph's stream.  Where that is the default stream, a backward
-// pass under capture would make it wait for the captured one, which ends the process: refused before.
+// A leaf that a living eager graph uses keeps its accumulation on that graph's stream, and what was computed eagerly goes back on its
+// own.  Where that is the default stream, a backward pass under capture would make it wait for the captured one, which ends the
+// process: refused before, for leaves and for everything that the operands were computed from.
 void refuse_eager_leaves(std::initializer_list<Maybe> tensors) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> kept;   // accumulators that only a weak reference holds
+    std::vector<torch::autograd::Node*> open;
+    std::unordered_set<torch::autograd::Node*> seen;
     for (const Maybe& t : tensors) {
-        if (!t || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!stream || stream->id() != 0, "a graph is being captured while an eager graph of the same leaf is alive on the default stream: "
+        if (!t || !t->defined() || !t->requires_grad()) continue;
+        kept.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+        open.push_back(kept.back().get());
+    }
+    while (!open.empty()) {
+        torch::autograd::Node* node = open.back();
+        open.pop_back();
+        if (!node || !seen.insert(node).second) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || stream->id() != 0, "a graph is being captured while an eager graph of the same leaf is alive on the default stream, or an operand was computed there: "
                     "let go of its results before, or warm up on another stream, or capture under no_grad");
+        for (const auto& edge : node->next_edges()) open.push_back(edge.function.get());
     }
 }
 

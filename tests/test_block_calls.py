@@ -260,3 +260,67 @@ def test_forward_mode_over_gradients_is_refused():
         with forward_ad.dual_level():   # a level without a tangent changes nothing
             got = entry(x)
         assert torch.equal(got, entry(x))
+
+
+# ------------------------------------------------------------------------------------------------------------- capture
+@pytest.mark.gpu
+def test_capture_looks_behind_views_and_results():
+    """Operands that were computed from a leaf of a living eager graph, or computed eagerly themselves.  Forward alone is captured; the
+    refusal comes before a backward pass could run."""
+    import strassen_hip as hip
+    f, _ = hip.rotary_frequencies(8)
+    p = torch.zeros(24, 8, device="cuda", requires_grad=True)
+    x = torch.zeros(3, 8, device="cuda")
+    calls = [lambda: hip.linear_act(x, p[:8]), lambda: hip.linear_act(p.view(3, 64)[:, :8], x), lambda: hip.linear_act(x, x, (p[0] * 2)[:3]), lambda: hip.linear_act(x, x, residual=p[:3, 5:]),
+             lambda: hip.layer_norm(x, p[1]), lambda: hip.layer_norm(torch.relu(p).sum(0)), lambda: hip.rotary(p.view(1, 4, 6, 8)[:, :, :4], None, f),
+             lambda: hip.rotary(x.view(1, 1, 3, 8), p[None, None, :2], f)[1]]
+    for call in calls:
+        alive = call()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        torch.cuda.synchronize()
+        del alive
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        g.replay()
+        torch.cuda.synchronize()
+        assert out.requires_grad
+        del out
+    eager = torch.relu(p[:3])   # no other graph of p is alive, but this operand's own way back is the default stream's
+    with pytest.raises(RuntimeError, match="computed there"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            hip.linear_act(eager, x)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_captured_gradients_through_views():
+    """A training step whose weights are parts of one packed leaf: captured, replayed four times with eager work between."""
+    import strassen_hip as hip
+    f, _ = hip.rotary_frequencies(8)
+    packed = _randn((64, 32), torch.bfloat16, 1, 0.2).cuda().requires_grad_()
+    x, dy = _randn((3, 5, 32), torch.bfloat16, 2).cuda(), _randn((3, 5, 32), torch.bfloat16, 3).cuda()
+
+    def step():
+        h = hip.layer_norm(x, packed[0], packed[1])
+        q = hip.rotary(hip.linear_act(h, packed[:32]).view(3, 5, 4, 8), None, f).reshape(3, 5, 32)
+        y = hip.linear_act(q, packed[32:], activation="silu", residual=h)
+        return y.detach(), torch.autograd.grad(y, packed, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(4):
+        x.copy_(_randn((3, 5, 32), torch.bfloat16, 20 + turn).cuda())
+        want = step()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
