@@ -10,6 +10,9 @@ namespace sthip {
 enum { TILE7_256 = 0, TILE7_128 = 1, TILE7_64 = 2, TILE7_32 = 3, TILE7_128_DEEP = 4, TILE7_256_128 = 5, TILE7_FEW_ROWS = 6 };
 inline int tile7_rows(int tile) { return tile == TILE7_256 || tile == TILE7_256_128 ? 256 : tile == TILE7_64 ? 64 : tile == TILE7_32 ? 32 : 128; }
 inline int tile7_cols(int tile) { return tile == TILE7_256 ? 256 : tile == TILE7_64 ? 64 : tile == TILE7_32 ? 32 : 128; }
+constexpr int tile7_threads(int tile) { return tile == TILE7_256 || tile == TILE7_256_128 ? 512 : 256; }
+// A launch holds less than 2^32 threads.
+constexpr bool launchable(int64_t workgroups, int threads) { return workgroups < ((int64_t)1 << 32) / threads; }
 // The tile that the debug switch (sthip_debug_force_tile) asks for, -1 if none.
 int debug_tile7();
 enum { LAYOUT_NT = 0, LAYOUT_NN = 1, LAYOUT_TN = 2 };   // both k-contiguous; B by its index; both by their index
@@ -21,15 +24,15 @@ typedef hipError_t (*LaunchPair7)(const Gemm7Pair& p, int tile, bool dma, hipStr
 extern const LaunchFn7 kForward7_0, kForward7_1, kForward7_2, kGradient7_0, kGradient7_1, kGradient7_2;
 extern const LaunchPair7 kPair7_0, kPair7_1, kPair7_2;
 
-// Whether the tile grid covers C and no tile lies outside of it, which the loaders' clamps rely on.
-inline bool covers(const Gemm7Params& p, int bm, int bn) {
-    return p.M > 0 && p.N > 0 && p.tiles_m == (p.M + bm - 1) / bm && p.tiles_n == (p.N + bn - 1) / bn && p.splits >= 1 && p.k_split > 0 &&
+// Whether the tile grid covers C and no tile lies outside of it, which the loaders' clamps rely on, and one launch holds it.
+inline bool covers(const Gemm7Params& p, int bm, int bn, int threads) {
+    return launchable((int64_t)p.tiles_m * p.tiles_n * p.splits, threads) && p.M > 0 && p.N > 0 && p.tiles_m == (p.M + bm - 1) / bm && p.tiles_n == (p.N + bn - 1) / bn && p.splits >= 1 && p.k_split > 0 &&
            (int64_t)p.k_split * p.splits >= p.K;
 }
 
 template <class T, int WM, int WN, int NWM, int NWN, int NS, bool A_KC, bool B_KC, bool DMA>
 hipError_t launch_gemm7_one(const Gemm7Params& p, hipStream_t stream) {
-    if (!covers(p, WM * NWM, WN * NWN)) return hipErrorInvalidValue;
+    if (!covers(p, WM * NWM, WN * NWN, NWM * NWN * 64)) return hipErrorInvalidValue;
     auto kern = gemm7_kernel<T, WM, WN, NWM, NWN, NS, A_KC, B_KC, DMA>;
     constexpr int smem_bytes = Pipe7<T, WM, WN, NWM, NWN, NS, A_KC, B_KC>::kSmem;
     static OptIn opted;
@@ -52,14 +55,16 @@ hipError_t launch_gemm7_layout(const Gemm7Params& p, int layout, hipStream_t str
 
 template <class T, int WM, int WN, int NWM, int NWN, int NS, bool DMA>
 hipError_t launch_gemm7_pair_one(const Gemm7Pair& p, hipStream_t stream) {
-    if (!covers(p.dx, WM * NWM, WN * NWN) || !covers(p.dw, WM * NWM, WN * NWN)) return hipErrorInvalidValue;
+    constexpr int threads = NWM * NWN * 64;
+    if (!covers(p.dx, WM * NWM, WN * NWN, threads) || !covers(p.dw, WM * NWM, WN * NWN, threads)) return hipErrorInvalidValue;
+    const int tiles = p.dx_tiles + p.dw.tiles_m * p.dw.tiles_n * p.dw.splits;
+    if (!launchable(tiles, threads)) return hipErrorInvalidValue;
     auto kern = gemm7_pair_kernel<T, WM, WN, NWM, NWN, NS, DMA>;
     constexpr int smem_bytes = Pipe7<T, WM, WN, NWM, NWN, NS, true, false>::kSmem;
     static OptIn opted;
     hipError_t e = opt_in_lds(opted, reinterpret_cast<const void*>(kern), smem_bytes);
     if (e != hipSuccess) return e;
-    const int tiles = p.dx_tiles + p.dw.tiles_m * p.dw.tiles_n * p.dw.splits;
-    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(NWM * NWN * 64), smem_bytes, stream, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(threads), smem_bytes, stream, p);
     return hipGetLastError();
 }
 

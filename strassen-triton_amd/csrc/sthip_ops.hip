@@ -49,16 +49,18 @@ double step_time(const TileCost& c, int dt, bool dma, int64_t q, int64_t workgro
     return c.rate[q - 1] * (dma ? 1.0 : c.through);
 }
 
-// Tile and splits of the k range by the sizes alone, so that the workspace query and the call agree: the cheapest by the table.
-// A split costs the joining launch (3 us) and its sums' way to memory and back.
+// Tile and splits of the k range by the sizes alone, so that the workspace query and the call agree: the cheapest by the table of
+// those whose workgroups one launch holds; tile -1 where there is none.  A split costs the joining launch (3 us) and its sums' way to
+// memory and back.
 Plan7 plan7(int64_t M, int64_t N, int64_t K, int dt, bool dma) {
     const int bk = 128 / elem_size(dt), forced = debug_tile7();
     const int64_t steps = std::max<int64_t>(1, ceil_div(K, bk));
-    Plan7 best = {TILE7_128, 1, (int)(steps * bk)};
+    Plan7 best = {-1, 1, (int)(steps * bk)};
     double least = 1e300;
     for (const TileCost& c : tiles_for(dt)) {
         if (!usable(c.tile, dt, dma) || passed_over(c.tile, dt, dma, forced)) continue;
         const int64_t tiles = ceil_div(M, tile7_rows(c.tile)) * ceil_div(N, tile7_cols(c.tile));
+        if (!launchable(tiles, tile7_threads(c.tile))) continue;   // splits are made of few tiles only
         for (int64_t s = 1; s <= 16; ++s) {
             if (s > 1 && (steps < 4 * s || tiles * (s - 1) >= kCus * c.held)) break;
             const int64_t per = ceil_div(steps, s), splits = ceil_div(steps, per), wgs = tiles * splits;
@@ -97,12 +99,13 @@ size_t product_workspace(int64_t M, int64_t N, int64_t K, int dt, bool forward) 
     return align256(most);
 }
 
-// The two products of a gradient as one launch: the same table over the tiles of both; dx takes sx splits, dW sw.
+// The two products of a gradient as one launch: the same table over the tiles of both; dx takes sx splits, dW sw.  Tile -1 where no
+// launch holds both.
 struct PlanPair { int tile; Plan7 dx, dw; };
 PlanPair plan_pair(int64_t rows, int64_t in, int64_t out, int dt, bool dma) {
     const int bk = 128 / elem_size(dt), forced = debug_tile7();
     const int64_t steps_x = std::max<int64_t>(1, ceil_div(out, bk)), steps_w = std::max<int64_t>(1, ceil_div(rows, bk));
-    PlanPair best = {};
+    PlanPair best = {-1, {-1, 1, 0}, {-1, 1, 0}};
     double least = 1e300;
     for (const TileCost& c : tiles_for(dt)) {
         if (!usable(c.tile, dt, dma) || passed_over(c.tile, dt, dma, forced)) continue;
@@ -114,6 +117,7 @@ PlanPair plan_pair(int64_t rows, int64_t in, int64_t out, int dt, bool dma) {
                 if (sw > 1 && (steps_w < 4 * sw || tw * (sw / 2) >= slots)) break;
                 const int64_t px = ceil_div(steps_x, sx), pw = ceil_div(steps_w, sw), nx = ceil_div(steps_x, px), nw = ceil_div(steps_w, pw);
                 const int64_t wgs = tx * nx + tw * nw, most = std::max(px, pw);
+                if (!launchable(wgs, tile7_threads(c.tile))) continue;
                 double t;
                 if (wgs <= slots) t = c.fixed + (double)most * step_time(c, dt, dma, std::max<int64_t>(1, ceil_div(wgs, kCus)), wgs);
                 else t = c.fixed * (double)ceil_div(wgs, slots) + step_time(c, dt, dma, c.held, wgs) * ((double)(tx * nx * px + tw * nw * pw) / slots + (wgs % slots ? 0.5 * (double)most : 0.0));
@@ -160,21 +164,17 @@ Gemm7Params product_params(const Operand& a, const Operand& b, void* C, int64_t 
     P.part = reinterpret_cast<float*>(ws);
     return P;
 }
-// Tile numbers and the joining launch's workgroups are 32-bit; 32 x 32 is the smallest tile, 16 the most splits.
-bool too_large(int64_t M, int64_t N) { return ceil_div(M, 32) * ceil_div(N, 32) * 16 >= 4 * kMaxSize; }
 int refuse_size(int64_t M, int64_t N, int64_t K) { return fail(STHIP_ERR_SHAPE, "product of %lld x %lld x %lld is too large", (long long)M, (long long)N, (long long)K); }
 
-int product(const Operand& a, const Operand& b, void* C, int64_t c_ld, int64_t M, int64_t N, int64_t K, int dt, const Epilogue& ep, void* ws, hipStream_t stream) {
-    if (M == 0 || N == 0) return STHIP_OK;
-    if (too_large(M, N)) return refuse_size(M, N, K);
-    const int es = elem_size(dt);
-    const bool dma = direct_loads(a, M, es) && direct_loads(b, N, es);
-    Plan7 pl = plan7(M, N, K, dt, dma);
-    if (a.kc && b.kc && few_rows(M, N, dt)) pl = plan_few(N, K, dt);
+bool product_direct(const Operand& a, const Operand& b, int64_t M, int64_t N, int dt) { return direct_loads(a, M, elem_size(dt)) && direct_loads(b, N, elem_size(dt)); }
+Plan7 plan_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, int dt) {
+    return a.kc && b.kc && few_rows(M, N, dt) ? plan_few(N, K, dt) : plan7(M, N, K, dt, product_direct(a, b, M, N, dt));
+}
+int product(const Plan7& pl, const Operand& a, const Operand& b, void* C, int64_t c_ld, int64_t M, int64_t N, int64_t K, int dt, const Epilogue& ep, void* ws, hipStream_t stream) {
     const int layout = a.kc ? (b.kc ? LAYOUT_NT : LAYOUT_NN) : LAYOUT_TN;
     const LaunchFn7 fn = layout == LAYOUT_NT ? (dt == STHIP_F32 ? kForward7_0 : dt == STHIP_F16 ? kForward7_1 : kForward7_2)
                                              : (dt == STHIP_F32 ? kGradient7_0 : dt == STHIP_F16 ? kGradient7_1 : kGradient7_2);
-    return launched(fn(product_params(a, b, C, c_ld, M, N, K, dt, ep, pl, ws), pl.tile, layout, dma, stream), "linear_act product");
+    return launched(fn(product_params(a, b, C, c_ld, M, N, K, dt, ep, pl, ws), pl.tile, layout, product_direct(a, b, M, N, dt), stream), "linear_act product");
 }
 
 int check_linear(int64_t rows, int64_t in, int64_t out, int dtype, int act) {
@@ -219,20 +219,36 @@ struct LaunchAct {
         else hipLaunchKernelGGL((act_backward_kernel<bf16_t, ACT>), grid, dim3(256), 0, s, a);
     }
 };
-template <class P> void launch_column_sum(const ColumnSumParams& c, int arrays, hipStream_t s) {
-    hipLaunchKernelGGL((column_sum_kernel<P>), dim3((unsigned)ceil_div(c.cols, 32), (unsigned)arrays), dim3(256), 0, s, c);
+// Eight threads a column, in launches of 2^24 columns (at 2^29 a launch would hold too many threads).
+template <class P> int column_sum(ColumnSumParams c, int arrays, hipStream_t s) {
+    const int64_t most = 1 << 24;
+    for (int64_t left = c.cols; left > 0; left -= most) {
+        c.cols = (int)std::min(left, most);
+        hipLaunchKernelGGL((column_sum_kernel<P>), dim3((unsigned)ceil_div(c.cols, 32), (unsigned)arrays), dim3(256), 0, s, c);
+        c.part += most;
+        for (void*& out : c.out) if (out) out = reinterpret_cast<P*>(out) + most;
+    }
+    return launched(hipGetLastError(), "column_sum");
 }
 int column_sum(const ColumnSumParams& c, int arrays, int dt, hipStream_t s) {
-    if (dt == STHIP_F32) launch_column_sum<float>(c, arrays, s);
-    else if (dt == STHIP_F16) launch_column_sum<f16_t>(c, arrays, s);
-    else launch_column_sum<bf16_t>(c, arrays, s);
-    return launched(hipGetLastError(), "column_sum");
+    return dt == STHIP_F32 ? column_sum<float>(c, arrays, s) : dt == STHIP_F16 ? column_sum<f16_t>(c, arrays, s) : column_sum<bf16_t>(c, arrays, s);
 }
 
 // ------------------------------------------------------------------ layer norm
 template <class T, class P, int TPR, int EPT, int RPB> void norm_forward(const NormParams& p, hipStream_t s) {
     const int64_t blocks = std::min<int64_t>(ceil_div(p.rows, RPB), kCus * (2048 / (TPR * RPB)));   // 2048 threads a CU
     hipLaunchKernelGGL((norm_forward_kernel<T, P, TPR, EPT, RPB>), dim3((unsigned)blocks), dim3(TPR * RPB), 0, s, p);
+}
+// Rows of 512 threads each, in launches of 2^16 rows (at 2^23 a launch would hold too many threads; 2 GiB of rows hide a launch).
+template <class T, class F> void long_rows(NormParams p, F&& launch) {
+    const int64_t most = 1 << 16;
+    for (int64_t left = p.rows; left > 0; left -= most) {
+        p.rows = (int)std::min(left, most);
+        launch(p);
+        auto on = [&](auto*& q, int64_t rs) { if (q) q = (T*)q + most * rs; };
+        on(p.x, p.x_rs), on(p.y, p.y_rs), on(p.dy, p.dy_rs), on(p.dx, p.dx_rs);
+        if (p.mean) p.mean += most, p.rstd += most;
+    }
 }
 template <class T, class P> void norm_forward_any(const NormParams& p, hipStream_t s) {
     if (p.cols <= 512) norm_forward<T, P, 64, 8, 4>(p, s);
@@ -241,7 +257,7 @@ template <class T, class P> void norm_forward_any(const NormParams& p, hipStream
     else if (p.cols <= 4096) norm_forward<T, P, 256, 16, 1>(p, s);
     else if (p.cols <= 8192) norm_forward<T, P, 512, 16, 1>(p, s);
     else if (p.cols <= 16384) norm_forward<T, P, 512, 32, 1>(p, s);
-    else hipLaunchKernelGGL((norm_forward_long_kernel<T, P>), dim3((unsigned)p.rows), dim3(512), 0, s, p);
+    else long_rows<T>(p, [&](const NormParams& r) { hipLaunchKernelGGL((norm_forward_long_kernel<T, P>), dim3((unsigned)r.rows), dim3(512), 0, s, r); });
 }
 constexpr int64_t kNormHeld = 16384;   // columns of the longest row that is held in registers
 // Threads a row and rows a workgroup of the gradient: 16 elements a thread up to 8192 columns (8 for short rows).
@@ -263,7 +279,7 @@ template <class T, class P> void norm_backward_any(const NormParams& p, hipStrea
     else if (p.cols <= 8192) norm_backward<T, P, 512, 16, 1>(p, s);
     else if (p.cols <= kNormHeld) norm_backward<T, P, 512, 32, 1>(p, s);
     else {
-        if (p.dx && p.rows > 0) hipLaunchKernelGGL((norm_backward_long_kernel<T, P>), dim3((unsigned)p.rows), dim3(512), 0, s, p);
+        if (p.dx) long_rows<T>(p, [&](const NormParams& r) { hipLaunchKernelGGL((norm_backward_long_kernel<T, P>), dim3((unsigned)r.rows), dim3(512), 0, s, r); });
         if (p.part) hipLaunchKernelGGL((norm_params_long_kernel<T>), dim3((unsigned)ceil_div(p.cols, 256), (unsigned)p.parts), dim3(256), 0, s, p);
     }
 }
@@ -318,8 +334,10 @@ int sthip_linear_act_forward(const void* x, const void* W, const void* bias, con
         (rc = check_stride("y", y_row_stride, out_features, rows)) || (residual && (rc = check_stride("residual", residual_row_stride, out_features, rows)))) return rc;
     if ((rc = check_workspace(workspace, workspace_bytes, sthip_linear_act_workspace_bytes(rows, in_features, out_features, dtype)))) return rc;
     const Epilogue ep = {bias, residual, residual ? residual_row_stride : 0, pre, activation};
-    return product({x, x_row_stride, true}, {W, w_row_stride, true}, y, y_row_stride, rows, out_features, in_features, dtype, ep, workspace,
-                   reinterpret_cast<hipStream_t>(stream));
+    const Operand a = {x, x_row_stride, true}, b = {W, w_row_stride, true};
+    const Plan7 pl = plan_product(a, b, rows, out_features, in_features, dtype);
+    if (pl.tile < 0) return refuse_size(rows, out_features, in_features);
+    return product(pl, a, b, y, y_row_stride, rows, out_features, in_features, dtype, ep, workspace, reinterpret_cast<hipStream_t>(stream));
 }
 
 size_t sthip_linear_act_backward_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int dtype, int activation) {
@@ -349,6 +367,16 @@ int sthip_linear_act_backward(const void* dy, const void* x, const void* W, cons
     int64_t dz_ld = dy_row_stride;
     const bool act = activation != STHIP_ACT_NONE;
     if (act) { dz = ws; dz_ld = N; ws += align256((size_t)M * N * es); }
+    // dx = dz W: W's rows are the k index; dW = dz^T x: both operands' rows are
+    const Operand rows_dz = {dz, dz_ld, true}, cols_dz = {dz, dz_ld, false}, w = {W, w_row_stride, false}, xo = {x, x_row_stride, false};
+    const bool has_dx = dx && M > 0 && K > 0, has_dw = dW && N > 0 && K > 0;
+    const bool dma = has_dx && has_dw && product_direct(rows_dz, w, M, K, dtype) && product_direct(cols_dz, xo, N, K, dtype);
+    const PlanPair pair = has_dx && has_dw ? plan_pair(M, K, N, dtype, dma) : PlanPair{-1, {}, {}};
+    Plan7 plan_x = {}, plan_w = {};
+    if (pair.tile < 0) {   // one by one; refused, if at all, before anything is launched
+        if (has_dx && (plan_x = plan_product(rows_dz, w, M, K, N, dtype)).tile < 0) return refuse_size(M, K, N);
+        if (has_dw && (plan_w = plan_product(cols_dz, xo, N, K, M, dtype)).tile < 0) return refuse_size(N, K, M);
+    }
     if (N > 0 && (dbias || (act && M > 0))) {
         const ActPlan pl = act_plan(M, N, dtype);
         ActParams a = {};
@@ -366,21 +394,16 @@ int sthip_linear_act_backward(const void* dy, const void* x, const void* W, cons
         }
     }
     const Epilogue none = {nullptr, nullptr, 0, nullptr, ACT_NONE};
-    // dx = dz W: W's rows are the k index; dW = dz^T x: both operands' rows are
-    if (dx && dW && M > 0 && K > 0 && N > 0) {
-        if (too_large(M, K) || too_large(N, K)) return refuse_size(M, K, N);
-        const Operand a = {dz, dz_ld, true}, at = {dz, dz_ld, false}, b = {W, w_row_stride, false}, c = {x, x_row_stride, false};
-        const bool dma = direct_loads(a, M, es) && direct_loads(at, N, es) && direct_loads(b, K, es) && direct_loads(c, K, es);
-        const PlanPair pl = plan_pair(M, K, N, dtype, dma);
+    if (pair.tile >= 0) {
         Gemm7Pair P;
-        P.dx = product_params(a, b, dx, K, M, K, N, dtype, none, pl.dx, ws);
-        P.dw = product_params(at, c, dW, K, N, K, M, dtype, none, pl.dw, ws + part_bytes(pl.dx, M, K));
+        P.dx = product_params(rows_dz, w, dx, K, M, K, N, dtype, none, pair.dx, ws);
+        P.dw = product_params(cols_dz, xo, dW, K, N, K, M, dtype, none, pair.dw, ws + part_bytes(pair.dx, M, K));
         P.dx_tiles = P.dx.tiles_m * P.dx.tiles_n * P.dx.splits;
         const LaunchPair7 fn = dtype == STHIP_F32 ? kPair7_0 : dtype == STHIP_F16 ? kPair7_1 : kPair7_2;
-        return launched(fn(P, pl.tile, dma, s), "linear_act gradient");
+        return launched(fn(P, pair.tile, dma, s), "linear_act gradient");
     }
-    if (dx && (rc = product({dz, dz_ld, true}, {W, w_row_stride, false}, dx, K, M, K, N, dtype, none, ws, s))) return rc;
-    if (dW && (rc = product({dz, dz_ld, false}, {x, x_row_stride, false}, dW, K, N, K, M, dtype, none, ws, s))) return rc;
+    if (has_dx && (rc = product(plan_x, rows_dz, w, dx, K, M, K, N, dtype, none, ws, s))) return rc;
+    if (has_dw && (rc = product(plan_w, cols_dz, xo, dW, K, N, K, M, dtype, none, ws, s))) return rc;
     return STHIP_OK;
 }
 

@@ -3,6 +3,7 @@
 //   buf NAME BYTES [FILE]     a 256-byte aligned buffer of exactly BYTES bytes, filled with 0xA5 or read from FILE
 //   save NAME FILE            write a buffer to FILE
 //   tile N                    the products' tile (the numbers of sthip_launch7.hpp), -1 = the table's choice
+//   dry                       from here on launches are printed (grid x, y, z, block x) instead of run; buffers may be called "@": a place that is never read
 //   late 0|1                  direct-to-LDS loads land at once, or not before the lane's wait lets them
 //   linear / linear_backward / norm / norm_backward / rotary ARGS...
 //                             the entry point of include/strassen_hip.h, arguments in its order without the stream; buffers by
@@ -32,6 +33,8 @@ int debug_tile7() { return g_tile; }
 
 struct Buf { char* p; size_t n; };
 static std::map<std::string, Buf> g_bufs;
+static std::vector<HostLaunch> g_launches;
+static char* const kNowhere = (char*)((uintptr_t)1 << 40);
 static char* alloc(size_t n) { void* p = nullptr; if (posix_memalign(&p, 256, n ? n : 1)) exit(2); memset(p, 0xA5, n); return (char*)p; }
 
 int main(int argc, char** argv) {
@@ -46,6 +49,7 @@ int main(int argc, char** argv) {
             std::string name;
             in >> name;
             if (name == "-") return nullptr;
+            if (name == "@" && g_host_dry) return kNowhere;
             const size_t plus = name.find('+');
             const size_t off = plus == std::string::npos ? 0 : std::stoull(name.substr(plus + 1));
             name = name.substr(0, plus);
@@ -55,7 +59,7 @@ int main(int argc, char** argv) {
         auto num = [&]() { long long v; if (!(in >> v)) { fprintf(stderr, "number expected: %s\n", line.c_str()); exit(2); } return (int64_t)v; };
         auto real = [&]() { double v; if (!(in >> v)) exit(2); return v; };
         Buf ws = {nullptr, 0};
-        auto scratch = [&](size_t n) { ws.n = n; if (n) ws.p = alloc(n); };
+        auto scratch = [&](size_t n) { ws.n = n; if (n) ws.p = g_host_dry ? kNowhere : alloc(n); };
         g_host_global.clear();
         int rc = 0;
         if (op == "buf") {
@@ -82,6 +86,7 @@ int main(int argc, char** argv) {
             continue;
         }
         if (op == "tile") { sthip::g_tile = (int)num(); continue; }
+        if (op == "dry") { g_host_dry = &g_launches; continue; }
         if (op == "late") { g_host_late = num() != 0; continue; }
         for (auto& kv : g_bufs) g_host_global.push_back({kv.second.p, kv.second.n});
         if (op == "linear") {
@@ -127,6 +132,13 @@ int main(int argc, char** argv) {
         } else {
             fprintf(stderr, "unknown statement %s\n", op.c_str());
             return 2;
+        }
+        if (g_host_dry) {
+            printf("%d", rc);
+            for (const HostLaunch& l : g_launches) printf(" %u,%u,%u,%u", l.grid[0], l.grid[1], l.grid[2], l.block[0]);
+            printf("\n");
+            g_launches.clear();
+            continue;
         }
         free(ws.p);
         if (rc) { fprintf(stderr, "%s returned %d\n", line.c_str(), rc); return 1; }

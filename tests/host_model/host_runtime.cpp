@@ -209,8 +209,11 @@ void host_mfma_32x32x2(float a_inst, float b_inst, float acc16[16]) {
 }
 
 
+std::vector<HostLaunch>* g_host_dry = nullptr;
+
 // One workgroup at a time, one thread per lane; the workgroup barrier is sized to the block.
 void host_launch(dim3 grid, dim3 block, const std::function<void()>& body) {
+    if (g_host_dry) { g_host_dry->push_back({{grid.x, grid.y, grid.z}, {block.x, block.y, block.z}}); return; }
     static bool init = false;
     if (!init) {
         for (auto& b : g_wave_barrier) pthread_barrier_init(&b, nullptr, kLanes);

@@ -324,3 +324,89 @@ def test_captured_gradients_through_views():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+# -------------------------------------------------------------------------------------------------- the largest sizes
+@pytest.fixture(scope="module")
+def cli(tmp_path_factory):
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_model"))
+    import hostbuild
+    if hostbuild.clang() is None:
+        pytest.skip("no clang to build the kernels for the host")
+    return hostbuild.build_block(str(tmp_path_factory.mktemp("calls")), "plain")
+
+
+def _launches(cli, tmp_path, lines):
+    """What each call would launch: (status, [(grid x, y, z, block x)])."""
+    import subprocess
+    script = tmp_path / "script"
+    script.write_text("\n".join(["dry"] + lines) + "\n")
+    r = subprocess.run([cli, str(script)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    out = [line.split() for line in r.stdout.splitlines()]
+    assert len(out) == len(lines)
+    return [(int(o[0]), [tuple(int(v) for v in launch.split(",")) for launch in o[1:]]) for o in out]
+
+
+M = (1 << 30) - 1
+ODD = 4099   # a row stride that no 16-byte chunk fits
+LARGE = [(M, 4, 1), (M, 4, 32), (1 << 29, 4, 33), (M, 8, 64), (M, 4, 127), ((1 << 29) - 31, 5, 17), (1, 4, M), (9, 8, M), (16, 3, 1 << 29), (17, 8, M), (40, 4, M), (1 << 20, 64, 1 << 16), (3, M, 2), (40, M, 1)]
+
+
+@pytest.mark.parametrize("code", [0, 1, 2])
+def test_no_launch_is_larger_than_the_hardware_takes(cli, tmp_path, code):
+    """Sizes up to 2^30 - 1, as far as a card's memory holds their operands: less than 2^32 threads in each direction of every launch, and
+    together no fewer workgroups than the sizes need."""
+    lines = []
+    for m, k, n in LARGE:
+        for pad in (0, ODD):
+            lines.append("linear @ @ @ @ @ @ %d %d %d %d %d %d %d %d 4" % (m, k, n, k + pad, k + pad, n + pad, n + pad, code))
+            for dx, dw in (("@", "@"), ("@", "-"), ("-", "@")):
+                lines.append("linear_backward @ @ @ @ %s %s @ %d %d %d %d %d %d %d 4" % (dx, dw, m, k, n, n + pad, k + pad, k + pad, code))
+    norms = [(M, 1), (1 << 23, 16385), ((1 << 23) + 5, 20000), (1, M), (1, 1 << 29), (70, 1 << 29), (M, 64)]
+    for rows, cols in norms:
+        lines.append("norm @ @ @ @ @ @ %d %d %d %d %d %d 1e-5" % (rows, cols, cols, cols, code, code))
+        lines.append("norm_backward @ @ @ @ @ @ @ @ %d %d %d %d %d %d %d" % (rows, cols, cols, cols, cols, code, code))
+    lines.append("rotary @ @ @ @ 1 %d 1 1 8 8 16 16 8 16 16 8 16 16 8 16 16 8 @ @ 64 0 1 0 1.0 0 0 %d" % (M, code))
+    got = _launches(cli, tmp_path, lines)
+    for line, (rc, launches) in zip(lines, got):
+        assert rc == 0 and launches, line
+        for gx, gy, gz, bx in launches:
+            assert gx * bx < 1 << 32 and gy < 1 << 16 and gz == 1 and bx <= 1024, (line, gx, gy, bx)
+    tail = got[8 * len(LARGE):]
+    for (rows, cols), (_, fwd), (_, bwd) in zip(norms, tail[::2], tail[1::2]):
+        sums = [g for g in bwd if g[1] == 2 and g[3] == 256][-(-(-cols // (1 << 24))):]
+        assert sum(g[0] for g in sums) == -(-cols // 32), (rows, cols)
+        if cols > 16384:
+            assert sum(g[0] for g in fwd) == rows and sum(g[0] for g in bwd if g[3] == 512) == rows, (rows, cols)
+
+
+def test_sizes_that_no_launch_holds_are_refused_before_any(cli, tmp_path):
+    """More tiles than a launch holds whichever tile is taken: nothing is launched, not the activation's gradient either."""
+    n = 1 << 20
+    got = _launches(cli, tmp_path, ["linear @ @ @ @ @ @ %d 8 %d 8 8 %d %d 1 4" % (n, n, n, n), "linear_backward @ @ @ @ @ - @ %d %d 8 8 %d %d 1 4" % (n, n, n, n),
+                                    "linear_backward @ @ @ @ - @ @ 8 %d %d %d %d %d 1 4" % (n, n, n, n, n)])
+    assert got == [(-1, [])] * 3
+
+
+@pytest.mark.gpu
+def test_norm_over_several_launches():
+    """Long rows and long column sums go in pieces: what lies on both sides of a border is what it is alone."""
+    import strassen_hip as hip
+    rows, cols = (1 << 16) + 3, 16389
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1)).requires_grad_()
+    w, b = (_randn((cols,), torch.float32, 2 + i).cuda() for i in range(2))
+    y = hip.layer_norm(x, w, b)
+    (dx,) = torch.autograd.grad(y, x, y.detach())
+    for at in (slice(0, 2), slice((1 << 16) - 2, rows)):
+        want = ref.norm(x[at].detach().cpu(), w.cpu(), b.cpu(), 1e-5, torch.bfloat16, torch.float32, y[at].detach().cpu())
+        ref.check(y[at].detach(), want["y"])
+        ref.check(dx[at], want["dx"])
+    del x, y, dx
+    cols = (1 << 24) + 37
+    x, dy = _randn((3, cols), torch.float32, 5), _randn((3, cols), torch.float32, 6)
+    gw, gb = (torch.ones(cols, device="cuda", dtype=torch.float32).requires_grad_() for _ in range(2))
+    hip.layer_norm(x.cuda(), gw, gb).backward(dy.cuda())
+    want = ref.norm(x, torch.ones(cols), torch.ones(cols), 1e-5, torch.float32, torch.float32, dy)
+    ref.check(gw.grad, want["dw"])
+    ref.check(gb.grad, want["db"])
