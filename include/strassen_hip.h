@@ -250,8 +250,8 @@ int sthip_layer_norm_backward(const void* dy, const void* x, const void* weight,
 /* Rotary positions (reference model/layers.py:59-118): of every head of q and k the pairs of the first rotary_dim elements
  * -- (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where `interleaved` -- are turned by position * frequencies[i] radians and
  * multiplied by `gain`; the elements behind them are copied.  k may be NULL.  Strides are {batch, token, head} in
- * elements, unit stride within a head; q_out may be q (and k_out k) with the same strides, and overlaps nothing
- * else.  `frequencies`: rotary_dim / 2 doubles in device memory.  `positions`: integers of positions_bits (32 or 64) in
+ * elements, unit stride within a head; q_out may be q (and k_out k) with the same strides (others are refused), and
+ * overlaps nothing else.  `frequencies`: rotary_dim / 2 doubles in device memory.  `positions`: integers of positions_bits (32 or 64) in
  * device memory at batch * positions_batch_stride + token * positions_token_stride, or NULL for first_position +
  * token.  Any position is allowed; the angle is formed in 64 bits.  inverse != 0 turns the other way, which is the
  * gradient's way back. */

@@ -476,6 +476,12 @@ int sthip_rotary(const void* q, const void* k, void* q_out, void* k_out,
     if (rows == 0 || heads == 0) return STHIP_OK;
     if (!frequencies || (q_heads > 0 && (!q || !q_out || !q_strides || !q_out_strides)) || (k_heads > 0 && (!k_out || !k_strides || !k_out_strides)))
         return fail(STHIP_ERR_ARG, "null pointer");
+    // in place with other strides a head would be written where another one is still to be read
+    auto moved = [&](const void* from, const void* to, const int64_t* a, const int64_t* b, int64_t n) {
+        return from == to && ((batch > 1 && a[0] != b[0]) || (tokens > 1 && a[1] != b[1]) || (n > 1 && a[2] != b[2]));
+    };
+    if ((q_heads > 0 && moved(q, q_out, q_strides, q_out_strides, q_heads)) || (k_heads > 0 && moved(k, k_out, k_strides, k_out_strides, k_heads)))
+        return fail(STHIP_ERR_LAYOUT, "rotary in place needs the same strides on both sides");
     RotaryParams p = {};
     p.q = q; p.k = k; p.qo = q_out; p.ko = k_out;
     p.freq = frequencies; p.pos = positions; p.pos64 = positions_bits == 64; p.pos_bs = positions_batch_stride; p.pos_ts = positions_token_stride; p.first = first_position;

@@ -410,3 +410,17 @@ def test_norm_over_several_launches():
     want = ref.norm(x, torch.ones(cols), torch.ones(cols), 1e-5, torch.float32, torch.float32, dy)
     ref.check(gw.grad, want["dw"])
     ref.check(gb.grad, want["db"])
+
+
+# ------------------------------------------------------------------------------------------------------------ the C ABI
+def test_rotary_in_place_with_other_strides_is_refused():
+    import ctypes
+    from strassen_hip import _capi
+    lib = _capi.load()
+    strides = lambda *v: (ctypes.c_int64 * 3)(*v)
+    here, there = ctypes.c_void_p(4096), ctypes.c_void_p(1 << 20)
+    call = lambda q, k, qo, ko, qs, ks, qos, kos, tokens=2: lib.sthip_rotary(q, k, qo, ko, 1, tokens, 2, 2, 8, 8, qs, ks, qos, kos, here, None, 0, 0, 0, 0, 1.0, 0, 0, 2, None)
+    packed, dense = strides(64, 32, 8), strides(32, 16, 8)
+    assert call(here, None, here, None, packed, None, dense, None) == -3 and b"same strides" in lib.sthip_last_error()
+    assert call(here, there, ctypes.c_void_p(8192), there, packed, packed, dense, dense) == -3
+    assert call(here, there, here, there, packed, packed, dense, dense, tokens=0) == 0
