@@ -6,7 +6,8 @@
 The fused kernel is instantiated once per (element type, algorithm) pair; the units
 plus the C-ABI front end compile in parallel and are linked into one shared library next to
 this file.  Object files go to csrc/build/ (git-ignored).  _sthip_torch.so beside it holds the
-torch side of the operators in csrc/sthip_torch.cpp (host code only, compiled by the host compiler).
+torch side of the operators in csrc/sthip_torch.cpp (host code only, compiled by the host compiler);
+where torch cannot be imported it is left out, and the library with its C ABI is built alone.
 """
 from __future__ import annotations
 
@@ -83,9 +84,12 @@ def _compile(unit, force):
 
 
 def _torch_commands():
-    """Compiling and linking the torch side; it links against the library, whose symbols it needs and whose code it does not."""
+    """Compiling and linking the torch side (None without torch); it links against the library, whose symbols it needs and whose code it does not."""
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
     from torch.utils.cpp_extension import include_paths, library_paths
     cxx, obj = os.environ.get("CXX", "g++"), os.path.join(OBJ, "sthip_torch.oo")
     compile_cmd = [cxx, "-O2", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_API_INCLUDE_EXTENSION_H",
@@ -118,8 +122,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
     jobs = jobs or min(8, os.cpu_count() or 1)
     units = _units()
     commands = _torch_commands()
-    torch_stamp, torch_digest = os.path.join(OBJ, "sthip_torch.sha"), _torch_digest(commands)
-    torch_new = force or not (os.path.exists(TORCH_LIB) and os.path.exists(torch_stamp) and open(torch_stamp).read() == torch_digest)
+    torch_stamp, torch_digest = os.path.join(OBJ, "sthip_torch.sha"), commands and _torch_digest(commands)
+    torch_new = commands and (force or not (os.path.exists(TORCH_LIB) and os.path.exists(torch_stamp) and open(torch_stamp).read() == torch_digest))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         torch_object = ex.submit(_run_torch, commands[0], "compiling") if torch_new else None
         results = list(ex.map(lambda u: _compile(u, force), units))
@@ -139,7 +143,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
         _run_torch(commands[1], "linking")
         open(torch_stamp, "w").write(torch_digest)
     if verbose:
-        print(TORCH_LIB, "built" if torch_new else "cached")
+        print(TORCH_LIB, "built" if torch_new else "cached" if commands else "left out: torch cannot be imported")
     return LIB
 
 

@@ -424,3 +424,17 @@ def test_rotary_in_place_with_other_strides_is_refused():
     assert call(here, None, here, None, packed, None, dense, None) == -3 and b"same strides" in lib.sthip_last_error()
     assert call(here, there, ctypes.c_void_p(8192), there, packed, packed, dense, dense) == -3
     assert call(here, there, here, there, packed, packed, dense, dense, tokens=0) == 0
+
+
+def test_the_library_is_built_without_torch(monkeypatch, capsys):
+    """Callers of the C ABI need no torch, neither does its build; the objects themselves are not compiled again here."""
+    import importlib.util
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("sthip_build", os.path.join(root, "strassen-triton_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    monkeypatch.setattr(build, "_compile", lambda unit, force: (unit[0], "cached"))
+    monkeypatch.setattr(build, "_run_torch", lambda cmd, what: pytest.fail("the torch side was built"))
+    monkeypatch.setitem(sys.modules, "torch", None)   # import torch raises ImportError
+    assert build.build() == build.LIB
+    assert "left out" in capsys.readouterr().out
