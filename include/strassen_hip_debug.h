@@ -42,8 +42,8 @@ int sthip_debug_one_launch_counters(const void* workspace, int64_t M, int64_t N,
 /* Overrides the tile table for later calls where the shape allows the forced tile: "128x128",
  * "256x128" (kernels that recombine in registers), "128x128g", "256x256" (grouped products),
  * "64x64" (fp32: seven products side by side on small tiles, sums formed in the operand loads);
- * for the products of sthip_linear_act_* "256x256", "256x128" (16-bit), "128x128", "128x128d" (four
- * stages), "64x64" and "32x32" (fp32); the setting must be the same for a workspace query and its call; NULL or anything else = automatic.  Returns the previous setting as a code (0 = automatic).
+ * for the products of sthip_linear_act_* "256x256", "256x128" and "128x128d" (16-bit; three and four
+ * stages), "128x128", "64x64" and "32x32" (fp32); the setting must be the same for a workspace query and its call; NULL or anything else = automatic.  Returns the previous setting as a code (0 = automatic).
  * The environment variable STHIP_FORCE_TILE gives the initial setting; it is read once, by the
  * first call into the library. */
 int sthip_debug_force_tile(const char* tile);

@@ -71,11 +71,10 @@ template <class T> __device__ __forceinline__ u32x4 load_chunk(const T* p, int n
     }
     return w;
 }
-template <class T> __device__ __forceinline__ void store_chunk(T* p, const u32x4& w, int n, int streaming = 0) {
+template <class T> __device__ __forceinline__ void store_chunk(T* p, const u32x4& w, int n) {
     constexpr int N = 16 / (int)sizeof(T);
     if (n >= N) {
-        any_u32x4* q = reinterpret_cast<any_u32x4*>(p);
-        if (streaming) __builtin_nontemporal_store((any_u32x4)w, q); else *q = w;
+        *reinterpret_cast<any_u32x4*>(p) = w;
         return;
     }
 #pragma unroll

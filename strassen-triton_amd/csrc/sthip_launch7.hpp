@@ -5,7 +5,7 @@
 
 namespace sthip {
 
-// 128_DEEP: four stages of LDS instead of two, one workgroup a CU; 256_128: 16-bit, three stages; 32: fp32 alone; the last is no
+// 128_DEEP: 16-bit, four stages of LDS instead of two, one workgroup a CU; 256_128: 16-bit, three stages; 32: fp32 alone; the last is no
 // tile but few_rows_kernel.
 enum { TILE7_256 = 0, TILE7_128 = 1, TILE7_64 = 2, TILE7_32 = 3, TILE7_128_DEEP = 4, TILE7_256_128 = 5, TILE7_FEW_ROWS = 6 };
 inline int tile7_rows(int tile) { return tile == TILE7_256 || tile == TILE7_256_128 ? 256 : tile == TILE7_64 ? 64 : tile == TILE7_32 ? 32 : 128; }
@@ -76,7 +76,7 @@ hipError_t launch_gemm7_pair(const Gemm7Pair& p, int tile, bool dma, hipStream_t
         case TILE7_128: e = dma ? launch_gemm7_pair_one<T, 64, 64, 2, 2, 2, true>(p, stream) : launch_gemm7_pair_one<T, 64, 64, 2, 2, 2, false>(p, stream); break;
         case TILE7_64: e = dma ? launch_gemm7_pair_one<T, 32, 32, 2, 2, 4, true>(p, stream) : launch_gemm7_pair_one<T, 32, 32, 2, 2, 2, false>(p, stream); break;
         case TILE7_256_128: if constexpr (sizeof(T) == 2) if (dma) e = launch_gemm7_pair_one<T, 64, 64, 4, 2, 3, true>(p, stream); break;
-        case TILE7_128_DEEP: if (dma) e = launch_gemm7_pair_one<T, 64, 64, 2, 2, 4, true>(p, stream); break;
+        case TILE7_128_DEEP: if constexpr (sizeof(T) == 2) if (dma) e = launch_gemm7_pair_one<T, 64, 64, 2, 2, 4, true>(p, stream); break;
         case TILE7_32: if constexpr (sizeof(T) == 4) e = dma ? launch_gemm7_pair_one<T, 16, 16, 2, 2, 4, true>(p, stream) : launch_gemm7_pair_one<T, 16, 16, 2, 2, 2, false>(p, stream); break;
     }
     if (e != hipSuccess || (p.dx.splits <= 1 && p.dw.splits <= 1)) return e;
@@ -101,7 +101,7 @@ hipError_t launch_gemm7(const Gemm7Params& p, int tile, int layout, bool dma, hi
         case TILE7_128: e = dma ? launch_gemm7_layout<FORWARD, T, 64, 64, 2, 2, 2, true>(p, layout, stream) : launch_gemm7_layout<FORWARD, T, 64, 64, 2, 2, 2, false>(p, layout, stream); break;
         case TILE7_64: e = dma ? launch_gemm7_layout<FORWARD, T, 32, 32, 2, 2, 4, true>(p, layout, stream) : launch_gemm7_layout<FORWARD, T, 32, 32, 2, 2, 2, false>(p, layout, stream); break;
         case TILE7_256_128: if constexpr (sizeof(T) == 2) if (dma) e = launch_gemm7_layout<FORWARD, T, 64, 64, 4, 2, 3, true>(p, layout, stream); break;
-        case TILE7_128_DEEP: if (dma) e = launch_gemm7_layout<FORWARD, T, 64, 64, 2, 2, 4, true>(p, layout, stream); break;
+        case TILE7_128_DEEP: if constexpr (sizeof(T) == 2) if (dma) e = launch_gemm7_layout<FORWARD, T, 64, 64, 2, 2, 4, true>(p, layout, stream); break;
         case TILE7_32: if constexpr (sizeof(T) == 4) e = dma ? launch_gemm7_layout<FORWARD, T, 16, 16, 2, 2, 4, true>(p, layout, stream) : launch_gemm7_layout<FORWARD, T, 16, 16, 2, 2, 2, false>(p, layout, stream); break;
     }
     if (e != hipSuccess || p.splits <= 1) return e;

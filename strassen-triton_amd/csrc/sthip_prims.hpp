@@ -24,8 +24,10 @@ __device__ __forceinline__ void lds_dma16_k(const void* sbase, uint32_t voff, ui
 }
 // The same under a lane mask that is all ones or zero: with no lane enabled the load is not executed
 // (no memory access, nothing to wait for).  Contract: the caller runs with all 64 lanes enabled, and
-// the statement leaves them enabled; it is only called from the k-loop of gemm4p_kernel, whose
-// control flow depends on blockIdx and kernel arguments alone.  exec is deliberately not in the
+// the statement leaves them enabled; it is only called from the k-loops of gemm4p_kernel and of Pipe7
+// (sthip_kernel7.hpp), whose workgroups are whole waves and whose control flow up to there depends on
+// blockIdx and kernel arguments alone (tile numbers, splits and steps come through readfirstlane, so that
+// the branches around the loop are scalar ones).  exec is deliberately not in the
 // clobber list: the statement restores the value the contract guarantees, and declaring it makes
 // the compiler fence every call with hazard nops and re-order the main loop around them.
 __device__ __forceinline__ void lds_dma16_km(const void* sbase, uint32_t voff, uint32_t lds_addr, int k, uint32_t mask) {
