@@ -438,3 +438,30 @@ def test_the_library_is_built_without_torch(monkeypatch, capsys):
     monkeypatch.setitem(sys.modules, "torch", None)   # import torch raises ImportError
     assert build.build() == build.LIB
     assert "left out" in capsys.readouterr().out
+
+
+# ------------------------------------------------------------------------------------------- infinities in the epilogue
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [3, 70])   # few rows; tiles
+def test_activations_and_slopes_at_the_ends(dt, name, rows):
+    """z of any size, infinities and NaN, by way of the bias: act(inf) = inf and slope 1, beyond the reach of exp on the other side 0
+    and slope 0 (relu exactly; the others' zero times -inf is NaN as in their formulas), NaN stays NaN."""
+    import strassen_hip as hip
+    inf, nan, big = float("inf"), float("nan"), 6e4 if dt == torch.float16 else 1e30
+    z = torch.tensor([inf, -inf, nan, big, -big, 120.0, -120.0, 0.0] * 9)
+    x, w = torch.zeros(rows, 24, dtype=dt).cuda(), _randn((72, 24), dt, 1).cuda()
+    b = z.to(dt).cuda().requires_grad_()
+    y = hip.linear_act(x, w, b, activation=name)
+    (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
+    low = z if name == "none" else torch.where(z < 0, torch.zeros(()), z)
+    if name not in ("none", "relu"):
+        low = torch.where(z == -inf, torch.tensor(nan), low)
+    slope = torch.ones(72) if name == "none" else torch.where(z == 0, torch.tensor(0.0 if name == "relu" else 0.5), (z > 0).float())
+    if name != "none":
+        slope = torch.where(z != z, z, slope)
+    y, db = y.detach().float().cpu(), db.float().cpu()
+    want = low.to(dt).float()
+    assert torch.equal(y.isnan(), want.isnan().expand(rows, 72)) and torch.equal(y.nan_to_num(1.0, 2e38, -2e38), want.nan_to_num(1.0, 2e38, -2e38).expand(rows, 72))
+    assert torch.equal(db.isnan(), slope.isnan()) and torch.equal(db.nan_to_num(7.0), (rows * slope).nan_to_num(7.0))   # sums of whole and half numbers: exact
