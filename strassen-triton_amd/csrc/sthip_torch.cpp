@@ -44,15 +44,17 @@ void require_gpu(const Tensor& t) {
     TORCH_CHECK(t.is_cuda(), "strassen_hip runs on MI355X tensors only (got a tensor on ", t.device(), "); there is no CPU implementation in this library");
 }
 // What torch would follow through its own operations and cannot follow into these: a tangent (forward-mode derivative), a transform's
-// wrapped tensor, a program that is being recorded.  All three would get a result as if it were a constant.
+// wrapped tensor or another one whose operations are dispatched elsewhere (its memory, if any, is not its value), a program that
+// is being recorded or run on tensors without memory.  All would get a result as if it were a constant, or none.
 template <class Tensors> void refuse_transforms(const Tensors& tensors) {
-    TORCH_CHECK(!torch::jit::tracer::isTracing() && !(c10::impl::TorchDispatchModeTLS::any_modes_set() &&
-                c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)), "the operators of strassen_hip cannot be traced");
+    auto mode = [](c10::impl::TorchDispatchModeKey k) { return c10::impl::TorchDispatchModeTLS::any_modes_set() && c10::impl::TorchDispatchModeTLS::get_mode(k); };
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !mode(c10::impl::TorchDispatchModeKey::PROXY) && !mode(c10::impl::TorchDispatchModeKey::FAKE),
+                "the operators of strassen_hip cannot be traced");
     const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Maybe& t : tensors) {
         if (!t || !t->defined()) continue;
-        TORCH_CHECK(!t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched})),
-                    "the operators of strassen_hip have no torch.func transforms");
+        TORCH_CHECK(!t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Python})) &&
+                    t->layout() == at::kStrided, "the operators of strassen_hip take plain tensors: no torch.func transforms, no subclass with operations of its own, no sparse ones");
         TORCH_CHECK(!tangents || !t->_fw_grad(0).defined(), "the operators of strassen_hip have no forward-mode derivatives");
     }
 }
@@ -71,14 +73,15 @@ struct On {
     explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-// A 2-D tensor the kernels can read: unit stride along columns, rows that do not overlap.
+// A 2-D tensor the kernels can read: unit stride along columns, rows that do not overlap, no pending negation.
 Tensor rows_of(const Tensor& t) {
+    if (t.is_neg()) return rows_of(t.resolve_neg());
     Tensor r = t.dim() == 2 ? t : t.reshape({t.dim() < 2 ? 1 : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), t.size(-1)});
     if (r.is_contiguous()) return r;
     if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < r.size(1))) return r.contiguous();
     return r;
 }
-Maybe contiguous(const Maybe& t) { return t && !t->is_contiguous() ? Maybe(t->contiguous()) : t; }
+Maybe contiguous(const Maybe& t) { return t && (t->is_neg() || !t->is_contiguous()) ? Maybe(t->resolve_neg().contiguous()) : t; }
 Tensor with_last(const Tensor& y, const Tensor& x, int64_t cols) {
     if (x.dim() == 2) return y;
     std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
@@ -294,7 +297,10 @@ void rotary_into(const Tensor& q, const Tensor& k, const Tensor& qo, const Tenso
                        freq.data_ptr<double>(), ptr(pos), given ? (int)pos->element_size() * 8 : 0, pos_batch, pos_token, h.first,
                        h.gain, (int)h.interleaved, inverse, dtype_code(q.scalar_type()), on.stream));
 }
-Tensor unit_heads(const Tensor& t) { return !t.defined() || t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+Tensor unit_heads(const Tensor& t) {
+    if (t.defined() && t.is_neg()) return unit_heads(t.resolve_neg());
+    return !t.defined() || t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous();
+}
 Tensor like(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; }
 
 struct Rotary : torch::autograd::Function<Rotary> {
@@ -411,12 +417,13 @@ std::tuple<Tensor, Maybe> rotary(const Tensor& q, const Maybe& k, const Tensor& 
                           "positions have shape ", pos->sizes(), ", expected [", tokens, "] or [", batch, ", ", tokens, "]");
     }
     TORCH_CHECK(!freq.requires_grad(), "rotary has no gradient for its frequencies");
-    const Tensor f = freq.contiguous();
+    const Tensor f = freq.resolve_neg().contiguous();
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k));
     if (inplace) {
         TORCH_CHECK(!grad, "rotary(inplace=True) has no gradient");
         for (const Tensor& t : {q4, k4}) {
             if (!t.defined()) continue;
+            TORCH_CHECK_VALUE(!t.is_neg(), "rotary(inplace=True) on a tensor with a pending negation");
             TORCH_CHECK_VALUE(t.size(3) <= 1 || t.stride(3) == 1, "rotary(inplace=True) needs unit stride within a head");
             TORCH_CHECK_VALUE(!overlaps_itself(t), "rotary(inplace=True) on a tensor whose elements share memory");
         }

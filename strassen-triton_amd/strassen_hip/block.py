@@ -6,7 +6,7 @@ Argument checks, memory and the autograd nodes are in csrc/sthip_torch.cpp (modu
 device memory, streams and the autograd graph only, and there is no CPU path.  Calls run on the current stream of their
 tensors' device; workspaces come from torch's allocator at every call, so captured graphs share none.  Wrong arguments raise
 ValueError or TypeError, a failing C-ABI call SthipError; gradients cannot be differentiated again.  Forward-mode derivatives,
-torch.func transforms and traces are refused (RuntimeError): the operators would count as constants in them.  Under capture, a
+torch.func transforms, traces and tensor subclasses are refused (RuntimeError): the operators would count as constants in them.  Under capture, a
 leaf that a living eager graph on the default stream uses is refused (RuntimeError), whether it is an operand or one was computed
 from it: torch's engine would end the process over it.
 """

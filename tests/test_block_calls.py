@@ -465,3 +465,51 @@ def test_activations_and_slopes_at_the_ends(dt, name, rows):
     want = low.to(dt).float()
     assert torch.equal(y.isnan(), want.isnan().expand(rows, 72)) and torch.equal(y.nan_to_num(1.0, 2e38, -2e38), want.nan_to_num(1.0, 2e38, -2e38).expand(rows, 72))
     assert torch.equal(db.isnan(), slope.isnan()) and torch.equal(db.nan_to_num(7.0), (rows * slope).nan_to_num(7.0))   # sums of whole and half numbers: exact
+
+
+# --------------------------------------------------------------------------------- tensors whose memory is not their value
+class _Counted(torch.Tensor):
+    """A tensor whose operations are its own; without memory."""
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+@pytest.mark.parametrize("i", range(9))
+def test_tensors_without_memory_are_refused(i):
+    import strassen_hip as hip
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    entry = _entries(hip, "cpu")[i]
+    x = _randn((4, 8), torch.float32, 1)
+    if i in (0, 1, 3, 4):   # the others take a part of x first, which is the subclass's own affair
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            entry(_Counted(x))
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            entry(x.to_sparse())
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(RuntimeError, match="cannot be traced"):
+        entry(x)
+
+
+@pytest.mark.gpu
+def test_pending_negations():
+    """The imaginary part of a conjugate is a view that is yet to be negated."""
+    import strassen_hip as hip
+    negative = lambda t: torch.complex(t, t).conj().imag
+    f, _ = hip.rotary_frequencies(8)
+    x, w, b, r = (_randn(s, torch.float32, i).cuda() for i, s in enumerate([(5, 1), (6, 1), (6,), (5, 6)]))
+    q = _randn((1, 4, 2, 16), torch.float32, 9).cuda()
+    same = lambda got, want: torch.equal(got, want)
+    assert negative(x).is_neg() and same(hip.linear_act(negative(x), w, b), hip.linear_act(-x, w, b))
+    assert same(hip.linear_act(x, negative(w), negative(b), residual=negative(r)), hip.linear_act(x, -w, -b, residual=-r))
+    assert same(hip.layer_norm(negative(r), negative(b), b), hip.layer_norm(-r, -b, b))
+    flat = torch._neg_view(q)
+    assert flat.is_neg() and flat.is_contiguous() and same(hip.rotary(flat, None, f), hip.rotary(-q, None, f)) and same(hip.layer_norm(flat), hip.layer_norm(-q))
+    with pytest.raises(ValueError, match="negation"):
+        hip.rotary(flat, None, f, inplace=True)
+    leaf = r.clone().requires_grad_()
+    y = hip.layer_norm(leaf, b)
+    assert same(torch.autograd.grad(y, leaf, torch._neg_view(r))[0], torch.autograd.grad(hip.layer_norm(leaf, b), leaf, -r)[0])
