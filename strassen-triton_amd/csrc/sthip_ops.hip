@@ -73,10 +73,15 @@ Plan7 plan7(int64_t M, int64_t N, int64_t K, int dt, bool dma) {
     }
     return best;
 }
-// Whether the forward product runs on few_rows_kernel.  16 rows, fp16 / bf16, few rows against tiles: N = 4096 11.1 / 16.7 us, 8192
-// 35.4 / 31.3, 16384 33.7 / 30.4; 8 rows, 16384: 28.6 / 30.1; fp32, whose tiles are bound by arithmetic: 67 / 95 at 16 rows.
+// Whether the forward product runs on few_rows_kernel.  Up to 4096 columns are a workgroup a CU; beyond, a second round begins, in
+// which each workgroup reads all of x again: with 9 to 16 rows the tiles are faster there.  Microseconds, few rows against the
+// best tile at k = 1024 / 4096 / 16384:
+//   16 rows, bf16:  N = 4096 4.4, 9.7, 37.9 against 6.4, 11.0, 33.1;  N = 16384 at k = 4096 33.7 against 30.4
+//   16 rows, fp32:  N = 4096 6.7, 19.3, 64.6 against 9.1, 18.9, 61.1;  N = 16384 18.9, 67.0, 256 against 13.4, 57.4, 191
+//    8 rows, bf16:  N = 4096 4.4, 8.7, 35.8 against 6.3, 10.7, 32.6;  N = 16384 8.3, 28.7, 113.5 against 7.6, 30.5, 113.9
+//    1 row,  fp32:  N = 4096 6.0, 18.0, 58.8 against 10.5, 18.1, 60.5;  N = 16384 16.9, 55.5, 206 against 13.2, 58.9, 190
 // Its launch takes 32 threads a column, of which there are less than 2^32.
-bool few_rows(int64_t M, int64_t N, int dt) { return debug_tile7() < 0 && N < (1 << 26) && (M <= 8 || (M <= 16 && (dt == STHIP_F32 || N <= 4096))); }
+bool few_rows(int64_t M, int64_t N) { return debug_tile7() < 0 && N < (1 << 26) && (M <= 8 || (M <= 16 && N <= 4096)); }
 // Its k range is split where that saves four turns of the eight waves, of 0.8 (16 bits, one row) to 1.4 us (fp32) each, against the
 // joining launch's 3 us; a workgroup a CU at most.  One range / split: 12 rows, 12224 -> 64 fp32 39.4 / 10.5 us, bf16 20.9 / 8.2; 1
 // row, 6144 -> 64 bf16 8.5 / 5.9; 16384 -> 2048 fp32 51.3 / 34.8, bf16 21.4 / 20.8.
@@ -88,7 +93,7 @@ Plan7 plan_few(int64_t N, int64_t K, int dt) {
 }
 size_t product_workspace(int64_t M, int64_t N, int64_t K, int dt, bool forward) {
     size_t most = 0;
-    if (forward && few_rows(M, N, dt)) {
+    if (forward && few_rows(M, N)) {
         const Plan7 p = plan_few(N, K, dt);
         return p.splits > 1 ? align256((size_t)p.splits * M * N * sizeof(float)) : 0;
     }
@@ -100,7 +105,9 @@ size_t product_workspace(int64_t M, int64_t N, int64_t K, int dt, bool forward) 
 }
 
 // The two products of a gradient as one launch: the same table over the tiles of both; dx takes sx splits, dW sw.  Tile -1 where no
-// launch holds both.
+// launch holds both.  With few rows, whose dW has less than a whole k-step, the table is off by up to a third: its choice against the
+// best tile, bias gradient included, 8 x 4096 -> 16384 bf16 76.5 / 75.0 us, fp32 201 / 175; 16 x 4096 -> 4096 bf16 32.8 / 32.3, fp32
+// 65.5 / 51.7; 13 x 5198 -> 12799 fp32 225 / 166; 13 x 1024 -> 4096 fp32 24.4 / 24.4.
 struct PlanPair { int tile; Plan7 dx, dw; };
 PlanPair plan_pair(int64_t rows, int64_t in, int64_t out, int dt, bool dma) {
     const int bk = 128 / elem_size(dt), forced = debug_tile7();
@@ -168,7 +175,7 @@ int refuse_size(int64_t M, int64_t N, int64_t K) { return fail(STHIP_ERR_SHAPE, 
 
 bool product_direct(const Operand& a, const Operand& b, int64_t M, int64_t N, int dt) { return direct_loads(a, M, elem_size(dt)) && direct_loads(b, N, elem_size(dt)); }
 Plan7 plan_product(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, int dt) {
-    return a.kc && b.kc && few_rows(M, N, dt) ? plan_few(N, K, dt) : plan7(M, N, K, dt, product_direct(a, b, M, N, dt));
+    return a.kc && b.kc && few_rows(M, N) ? plan_few(N, K, dt) : plan7(M, N, K, dt, product_direct(a, b, M, N, dt));
 }
 int product(const Plan7& pl, const Operand& a, const Operand& b, void* C, int64_t c_ld, int64_t M, int64_t N, int64_t K, int dt, const Epilogue& ep, void* ws, hipStream_t stream) {
     const int layout = a.kc ? (b.kc ? LAYOUT_NT : LAYOUT_NN) : LAYOUT_TN;

@@ -513,3 +513,14 @@ def test_pending_negations():
     leaf = r.clone().requires_grad_()
     y = hip.layer_norm(leaf, b)
     assert same(torch.autograd.grad(y, leaf, torch._neg_view(r))[0], torch.autograd.grad(hip.layer_norm(leaf, b), leaf, -r)[0])
+
+
+# ---------------------------------------------------------------------------------------- the borders of few rows' own way
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,d_in,d_out", [(8, 200, 4112), (9, 200, 4096), (9, 200, 4097), (16, 136, 5120), (16, 2051, 4100), (17, 200, 4096)])
+def test_few_rows_on_both_sides_of_their_borders(dt, rows, d_in, d_out):
+    import strassen_hip as hip
+    x, w, b, r = (_randn(s, dt, 30 + i, std) for i, (s, std) in enumerate([((rows, d_in), 1.0), ((d_out, d_in), d_in ** -0.5), ((d_out,), 1.0), ((rows, d_out), 1.0)]))
+    y = hip.linear_act(x.cuda(), w.cuda(), b.cuda(), activation="silu", residual=r.cuda())
+    ref.check(y, ref.linear(x, w, b, r, "silu", dt)["y"])
