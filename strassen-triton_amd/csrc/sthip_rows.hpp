@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(TPR * RPB) norm_forward_kernel(const NormParam
     }
 }
 
-// Rows too long for registers: the same three sweeps over the row, the second and third out of the caches.
+// Rows too long for registers: the same three sweeps over the row, the second and third out of the caches.  A workgroup a row: MI355X,
+// 4096 x 20000 bf16 111 us against 64 of bytes, 1024 x 65536 fp32 211 against 105, 16 x 131072 bf16 33 (16 workgroups).
 template <class T, class P>
 __global__ void __launch_bounds__(512) norm_forward_long_kernel(const NormParams p) {
     constexpr int N = Chunk<T>::N, TPR = 512;
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(512) norm_forward_long_kernel(const NormParams
 // RPB groups of TPR threads a workgroup, each walks the rows group, group + groups, ...: x and dy are read once, the next row's
 // chunks while this row is summed, and a group's share of dw and db stays in registers until its last row.  The groups of a
 // workgroup join theirs in LDS, the workgroups' shares are joined by column_sum_kernel: fp32 sums in a fixed order.  Bound by
-// memory: MI355X, 8192 x 4096 bf16 47 us = 4.3 TB/s and 4 us of joining; 4999 x 1537 fp32 26.7 us = 3.5 TB/s.
+// memory: MI355X, 8192 x 4096 bf16 47 us = 4.3 TB/s and 4 us of joining; 4999 x 1537 fp32 26.7 us = 3.5 TB/s (a quarter of the threads'
+// 2048 places is empty, and of the three turns that 512 workgroups of four rows make the last one is 44 % full).
 template <class T, class P, int TPR, int EPT, int RPB>
 __global__ void __launch_bounds__(TPR * RPB) norm_backward_kernel(const NormParams p) {
     constexpr int N = Chunk<T>::N, NV = EPT / N, WAVES = TPR * RPB / 64;
@@ -306,7 +308,8 @@ __global__ void __launch_bounds__(TPR * RPB) norm_backward_kernel(const NormPara
     }
 }
 
-// Rows too long for registers: dx alone, a workgroup a row, ...
+// Rows too long for registers: dx alone, a workgroup a row, two sweeps (with dw and db: 4096 x 20000 bf16 241 us against 96 of bytes,
+// 1024 x 65536 fp32 364 against 157), ...
 template <class T, class P>
 __global__ void __launch_bounds__(512) norm_backward_long_kernel(const NormParams p) {
     constexpr int N = Chunk<T>::N, TPR = 512;
@@ -379,7 +382,10 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const ColumnSumParams p
 }
 
 // dz = dy act'(pre), and the column sums of dz (the bias gradient) from the values before they are rounded.  A workgroup
-// takes 32 chunks of columns and a strip of rows, eight rows at a time, the next eight on their way meanwhile.  Bound by memory:
+// takes 32 chunks of columns and a strip of rows, eight rows at a time, the next eight on their way meanwhile.
+// dz leaves in the operand type, since the matrix cores read it twice: with bf16 that is 1.66e-3 of dx and dW, as much as their own
+// rounding; pre, rounded as well, adds 0.55e-3 (together 2.41e-3 against 1.66e-3).  In two terms of 16 bits dz would cost both
+// products twice, and pre in fp32 alone, at twice its bytes, would gain 3 % of the error.  Bound by memory:
 // MI355X, 8192 x 8192 bf16 gelu 84 us = 4.8 TB/s (without the next rows ahead 93).
 struct ActParams {
     const void* dy; const void* pre; void* dz;   // without an activation the sums alone: dz = dy
