@@ -93,7 +93,8 @@ Tensor with_last(const Tensor& y, const Tensor& x, int64_t cols) {
 Tensor restored(const Tensor& t, const char* what, at::IntArrayRef sizes, at::ScalarType type, const Tensor& grad) {
     TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == grad.device(), "the saved ", what, " came back as ", t.toString(), " of ",
                 t.sizes(), " on ", t.device(), ", expected ", type, " of ", sizes, " on ", grad.device());
-    return t;
+    refuse_transforms(variable_list{t});
+    return t.resolve_neg();
 }
 
 // What a backward pass returns, where it was asked for a graph of itself: tensors that refuse to be differentiated again.

@@ -182,6 +182,14 @@ def test_saved_tensors_come_back_otherwise(name):
             assert torch.equal(got, ref_)
     for got, ref_ in zip(torch.autograd.grad(checkpoint(lambda _: call(), leaves[0], use_reentrant=False), leaves, dy), want):
         assert torch.equal(got, ref_)
+    with saved_tensors_hooks(keep, lambda t: torch._neg_view(-t) if t.dtype.is_floating_point else t):
+        y = call()
+    for got, ref_ in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(got, ref_)
+    with saved_tensors_hooks(keep, _Counted):
+        y = call()
+    with pytest.raises(RuntimeError):   # the subclass's own refusal of an operation, or "plain tensors"
+        torch.autograd.grad(y, leaves, dy)
     for spoil in (lambda t: t.cpu(), lambda t: t[..., :1] if t.shape[-1] > 1 else t, lambda t: t.float() if t.dtype == torch.float64 else t.double()):
         with saved_tensors_hooks(keep, spoil):
             y = call()
