@@ -420,6 +420,26 @@ def test_norm_over_several_launches():
     ref.check(gb.grad, want["db"])
 
 
+@pytest.mark.gpu
+def test_more_rows_than_small_tiles_hold():
+    """2^29 rows and one output, forward and gradients: as 32 x 32 tiles they would be 2^32 threads."""
+    import strassen_hip as hip
+    rows = (1 << 29) + 5
+    x = torch.empty(rows, 4, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1)).requires_grad_()
+    w = _randn((1, 4), torch.float32, 2).cuda().requires_grad_()
+    y = hip.linear_act(x, w, activation="relu")
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones((), device="cuda").expand(rows, 1))
+    for at in (slice(0, 40), slice((1 << 28) - 20, (1 << 28) + 20), slice(rows - 40, rows)):
+        xs = x[at].detach().cpu()
+        want = ref.linear(xs, w.detach().cpu(), None, None, "relu", torch.float32, torch.ones(40, 1))
+        ref.check(y[at].detach(), want["y"])
+        ref.check(dx[at], want["dx"])
+    # dw: a sum of 2^29 products; with splits and k-steps in fp32, n steps of the sum of magnitudes at most, sqrt(n) of them in earnest
+    want = sum((piece.detach() * (piece.detach() @ w.detach().t() > 0)).double().sum(0) for piece in x.split(1 << 26))
+    size = sum(piece.detach().abs().double().sum(0) for piece in x.split(1 << 26))
+    assert ((dw[0].double() - want).abs() <= 2.0 ** 15 * ref.STEP * size).all(), (dw, want)
+
+
 # ------------------------------------------------------------------------------------------------------------ the C ABI
 def test_rotary_in_place_with_other_strides_is_refused():
     import ctypes
